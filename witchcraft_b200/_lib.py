@@ -1,4 +1,4 @@
-"""ctypes binding of the native library (include/wc_t5cuda.h, include/wc_codec.h).
+"""ctypes binding of the native library (include/*.h).
 
 The library is built in-tree by `witchcraft_b200.build`; loading fails loudly
 when it is missing.  There is no CPU fallback anywhere in this package.
@@ -66,6 +66,19 @@ _SIGNATURES = {
     "wc_q4_table": (c_int, [c_void_p]),
     "wc_similarities": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p]),
     "wc_query_last_error": (ctypes.c_char_p, []),
+    "wc_fp8_quantize_rows": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                     c_void_p]),
+    "wc_fp8_quantize_weight": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                       c_int64, c_void_p]),
+    "wc_fp8_rmsnorm": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p,
+                               c_int64, c_int64, ctypes.c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "wc_fp8_matmul": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                              c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64, c_void_p]),
+    "wc_fp8_gated_matmul": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64,
+                                    c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p,
+                                    c_int, c_int64, c_void_p, c_int64, c_void_p]),
+    "wc_fp8_sync": (c_int, [c_void_p]),
+    "wc_fp8_last_error": (ctypes.c_char_p, []),
 }
 
 

@@ -1,0 +1,109 @@
+// Shared by the 8-bit operators (fp8_rows.cu, fp8_gemm.cu): element types,
+// the e4m3 conversion and the scale of a block.
+#pragma once
+#include "common.cuh"
+
+#include "../../include/wc_fp8.h"
+
+namespace wc {
+
+constexpr int kFp8Block = 128;      // columns (and weight rows) that share a scale
+constexpr float kE4M3Max = 448.0f;  // largest finite e4m3 value
+
+// The scale of a block whose largest magnitude is amax (NaN stays NaN), and
+// what its values are multiplied by.  The floor keeps the reciprocal finite;
+// a block of zeros gets codes of zero.  inf: scale inf, factor 0, so finite
+// values become 0 * inf and infinite ones NaN codes.
+__device__ __forceinline__ float fp8_scale(float amax) {
+  const float s = amax * (1.0f / kE4M3Max);
+  return s < 1.17549435e-38f ? 1.17549435e-38f : s;
+}
+__device__ __forceinline__ float fp8_factor(float scale) { return __fdividef(1.0f, scale); }
+
+// Maximum that keeps a NaN (fmaxf drops it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+// max_nan over the warp, in every lane.
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float d;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+  return d;
+}
+
+// Four f32 -> four e4m3 bytes (first in the low byte), nearest even, saturating.
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+}
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Four consecutive elements at p (of a row with `left` elements from p on) as
+// f32, zeros past the row's end.  vec: p is aligned to four elements.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p, int64_t left, bool vec) {
+  if (vec && left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      return *reinterpret_cast<const float4*>(p);
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      const T* e = reinterpret_cast<const T*>(&u);
+      return make_float4(to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3]));
+    }
+  }
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (left > 0) v.x = to_f32(p[0]);
+  if (left > 1) v.y = to_f32(p[1]);
+  if (left > 2) v.z = to_f32(p[2]);
+  if (left > 3) v.w = to_f32(p[3]);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int64_t left, bool vec, float4 v) {
+  if (vec && left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(p) = v;
+    } else {
+      T e[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(e);
+    }
+    return;
+  }
+  if (left > 0) p[0] = from_f32<T>(v.x);
+  if (left > 1) p[1] = from_f32<T>(v.y);
+  if (left > 2) p[2] = from_f32<T>(v.z);
+  if (left > 3) p[3] = from_f32<T>(v.w);
+}
+// Four code bytes at p (4-byte aligned) of a row with `left` columns from p on.
+__device__ __forceinline__ void store_codes4(uint8_t* p, int64_t left, uint32_t c) {
+  if (left >= 4) {
+    *reinterpret_cast<uint32_t*>(p) = c;
+    return;
+  }
+  for (int i = 0; i < 3; ++i)
+    if (left > i) p[i] = static_cast<uint8_t>(c >> (8 * i));
+}
+
+// Host side: whether rows of `ld` elements from p are aligned to four
+// elements of `size` bytes.
+inline bool aligned4(const void* p, int64_t ld, int size) {
+  return (reinterpret_cast<uintptr_t>(p) % (4 * size)) == 0 && ld % 4 == 0;
+}
+inline int fp8_type_size(int t) { return t == WC_T_F32 ? 4 : t == WC_T_E4M3 ? 1 : 2; }
+
+}  // namespace wc

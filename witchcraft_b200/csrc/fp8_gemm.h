@@ -1,0 +1,28 @@
+// Host-visible launcher of the 8-bit tcgen05 products (fp8_gemm.cu).
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace wc {
+
+struct Fp8GemmParams {
+  const uint8_t *a, *w, *up;         // codes [m][lda], [n][ldw], [n][ldup] (up: gated only)
+  const float *sa, *sw, *sup;        // scales [m][ldsa], [n / 128][ldsw], [n / 128][ldsup]
+  const void* residual;              // [m][ldr] of the output's type, or null
+  void* out;                         // [m][ldo]
+  float* out_scales;                 // [m][ldos], 8-bit output only
+  int64_t lda, ldw, ldup, ldsa, ldsw, ldsup, ldr, ldo, ldos;
+  int m, n, k;
+  int act;                           // WC_ACT_*, gated only
+  bool vec_o, vec_r;                 // output / residual rows aligned to four elements
+  uint32_t* status;                  // wait timeouts; null: the library's own word
+};
+
+// out_type WC_T_E4M3 only with gated.
+cudaError_t fp8_gemm_launch(bool gated, int out_type, const Fp8GemmParams& p, int num_sms, cudaStream_t st);
+
+// The library's own status word on the current device, read and cleared.
+cudaError_t fp8_gemm_take_status(uint32_t* status);
+
+}  // namespace wc
