@@ -24,7 +24,8 @@ int done(cudaError_t e, const char* what) {
   return WC_E_CUDA;
 }
 
-constexpr int64_t kMaxSize = 0x7FFFFF00;  // rows, columns and weight rows are 32-bit inside the products
+constexpr int64_t kMaxSize = 0x7FFFFF00;  // rows and weight rows are 32-bit inside the products
+constexpr int64_t kMaxK = 1 << 30;        // columns: the row kernels add a few blocks to 32-bit column numbers
 
 bool value_type(int t) { return t == WC_T_F32 || t == WC_T_F16 || t == WC_T_BF16; }
 int type_size(int t) { return t == WC_T_F32 ? 4 : t == WC_T_E4M3 ? 1 : 2; }
@@ -74,7 +75,7 @@ int sm_count(int* n) {
 
 int quantize(bool weight, const void* x, int type, int64_t m, int64_t k, int64_t ldx, void* codes, int64_t ldc,
              float* scales, int64_t lds, void* stream) {
-  if (m < 0 || m > kMaxSize || k < 1 || k > kMaxSize) return refuse(WC_E_INVALID_ARG, "sizes out of range (m >= 0, k >= 1)");
+  if (m < 0 || m > kMaxSize || k < 1 || k > kMaxK) return refuse(WC_E_INVALID_ARG, "sizes out of range (m >= 0, k >= 1)");
   if (!value_type(type)) return refuse(WC_E_INVALID_ARG, "type must be f32, f16 or bf16");
   if (m == 0) return WC_OK;
   const char* bad = check_values(x, type, ldx, k);
@@ -118,7 +119,7 @@ int product(Fp8GemmParams& p, const void* a, int64_t lda, const float* sa, int64
 }
 
 bool sizes_ok(int64_t m, int64_t k, int64_t n) {
-  return m >= 0 && m <= kMaxSize && k >= 1 && k <= kMaxSize && n >= 1 && n <= kMaxSize;
+  return m >= 0 && m <= kMaxSize && k >= 1 && k <= kMaxK && n >= 1 && n <= kMaxSize;
 }
 
 }  // namespace
@@ -138,7 +139,7 @@ extern "C" int wc_fp8_quantize_weight(const void* d_w, int w_type, int64_t n, in
 extern "C" int wc_fp8_rmsnorm(const void* d_x, int x_type, int64_t ldx, const void* d_delta, int delta_type,
                               int64_t ldd, void* d_sum, int64_t ldsum, const float* d_w, int64_t m, int64_t k,
                               float eps, void* d_codes, int64_t ldc, float* d_scales, int64_t lds, void* stream) {
-  if (m < 0 || m > kMaxSize || k < 1 || k > kMaxSize) return refuse(WC_E_INVALID_ARG, "sizes out of range (m >= 0, k >= 1)");
+  if (m < 0 || m > kMaxSize || k < 1 || k > kMaxK) return refuse(WC_E_INVALID_ARG, "sizes out of range (m >= 0, k >= 1)");
   if (!(eps >= 0.0f)) return refuse(WC_E_INVALID_ARG, "eps must not be negative");
   if (!value_type(x_type)) return refuse(WC_E_INVALID_ARG, "type must be f32, f16 or bf16");
   if (m == 0) return WC_OK;

@@ -1,26 +1,34 @@
-// 8-bit products on the tensor cores (tcgen05 kind::f8f6f4), 128-row tiles.
+// 8-bit products on the tensor cores (tcgen05 kind::f8f6f4).
 //
 //   y[m][n] = sum_b sa[m][b] sw[n / 128][b] P_b[m][n],
 //   P_b[m][n] = sum over the 128 columns k of block b of qa[m][k] qw[n][k]
 //
 // The scales change with every block of 128 columns, so the tensor core's
 // accumulator cannot run over the whole of K: each block's P_b goes to one of
-// two TMEM buffers, and the epilogue warps add scale * P_b to sums that they
-// keep in registers (one multiply-add per element and block, packed in
-// pairs) while the tensor core fills the other buffer.
+// a few TMEM buffers, and the epilogue warps add scale * P_b to sums that they
+// keep in registers (one multiply-add per element and block, packed in pairs)
+// while the tensor core fills the next buffer.  A thread of the epilogue owns
+// one row (a TMEM lane) and half of the tile's columns, so its row scale is
+// one register and the weight scale of its columns one value per block.
+// For the gated product the 256 columns of a tile are 64 gate features, the
+// same 64 up features, the next 64 gate and the next 64 up: a thread holds
+// both factors of its 64 results.
 //
-// Tile: 128 rows x 256 columns.  A thread of the epilogue owns one row (a
-// TMEM lane) and 128 columns, so its row scale is one register and the weight
-// scale of its columns one value per block.  For the gated product the 256
-// columns are 64 gate, the same 64 up, the next 64 gate and up features, so a
-// thread holds both factors of its 64 results.
+// Two kernels:
+//   fp8_pair_kernel  many rows: persistent, 256 x 256 tiles on pairs of SMs,
+//                    results from registers through a small staging buffer
+//   fp8_tile_kernel  few rows: one 128-row tile per CTA or, with K split, per
+//                    cluster, whose CTAs join their sums through distributed
+//                    shared memory in rank order
 //
-// Warps (384 threads):
-//   0      TMA producer: 128 rows of codes and 256 weight rows per block,
-//          128-byte swizzle, ring of kStages
-//   1      TMEM allocation, MMA issue (one thread)
-//   4-11   epilogue: warp w reads TMEM lanes 32 (w % 4).., columns
-//          128 (w / 4 - 1)..
+// Warps of both (384 threads):
+//   0      TMA producer, 128-byte swizzle, ring of operand stages
+//   1      TMEM allocation, MMA issue (one thread; of the even CTA of a pair)
+//   4-11   epilogue: warp w reads TMEM lanes 32 (w % 4).., and the column
+//          half w / 4 - 1
+// Registers: 168 a thread at launch; the first four warps give back all but
+// 56 and the epilogue takes 224 (4 x 32 x 56 + 8 x 32 x 224 = 384 x 168).
+#include "cluster.cuh"
 #include "fp8.cuh"
 #include "fp8_gemm.h"
 
@@ -31,37 +39,44 @@ namespace wc {
 
 namespace {
 
-constexpr int kBM = 128;
-constexpr int kBN = 256;
-constexpr int kStages = 4;
-constexpr int kABytes = kBM * kFp8Block;
-constexpr int kBBytes = kBN * kFp8Block;
-constexpr int kStageBytes = kABytes + kBBytes;
-constexpr int kStageOutBytes = 32 * 128;  // one warp's 32 rows x 32 f32 on the way out
-constexpr int kOffOut = kStages * kStageBytes;
-constexpr int kOffAmax = kOffOut + 8 * kStageOutBytes;
-constexpr int kOffBar = kOffAmax + 2 * kBM * 4;
-constexpr int kSmem = 1024 + kOffBar + 256;
-static_assert(kSmem <= 232448, "dynamic shared memory per block");
+constexpr int kRows = 128;      // rows of a CTA's tile (TMEM lanes)
 constexpr int kThreads = 384;
-constexpr uint32_t kTmemCols = 512;  // two 256-column partials
+constexpr uint32_t kTmemCols = 512;
+constexpr int kABytes = kRows * kFp8Block;
 
 __device__ uint32_t g_fp8_status;  // wait timeouts of launches without a status word of their own
 
-// D[tmem] (+)= A[smem] . B[smem]^T for 8-bit floats, f32 accumulate, one CTA.
-__device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                          uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
 // Instruction descriptor for kind::f8f6f4 with e4m3 A and B (format 0), f32
 // D, both K-major.
 __host__ __device__ constexpr uint32_t idesc_e4m3_f32(int m, int n) {
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+// D[tmem] (+)= A[smem] . B[smem]^T for 8-bit floats, f32 accumulate.
+template <bool PAIR>
+__device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// One block of 128 columns: four MMAs of 32.
+template <bool PAIR>
+__device__ __forceinline__ void mma_block(uint32_t d_tmem, uint32_t a_smem, uint32_t b_smem, uint32_t idesc) {
+  const uint64_t adesc = sw128_kmajor_desc(a_smem), bdesc = sw128_kmajor_desc(b_smem);
+#pragma unroll
+  for (int k = 0; k < kFp8Block / 32; ++k)
+    tc_mma_f8<PAIR>(d_tmem, adesc + 2 * k, bdesc + 2 * k, idesc, k > 0 ? 1u : 0u);
 }
 
 // 32 lanes x 32 columns of f32: issue, and wait for everything issued.  The
@@ -88,34 +103,88 @@ __device__ __forceinline__ void tmem_ld32_wait(uint32_t (&r)[32]) {
                : "memory");
 }
 
+// acc[] (column pairs) += s0 * (first half) or s1 * (second half) of the
+// 32 CHUNKS columns at taddr; calls `read` once all of them are in registers.
+template <int CHUNKS, typename Read>
+__device__ __forceinline__ void add_block(uint32_t taddr, float s0, float s1, uint64_t (&acc)[16 * CHUNKS], Read read) {
+  uint32_t r[2][32];
+  tmem_ld32_issue(taddr, r[0]);
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    tmem_ld32_wait(r[c & 1]);
+    if (c + 1 < CHUNKS)
+      tmem_ld32_issue(taddr + 32 * (c + 1), r[(c + 1) & 1]);
+    else
+      read();
+    const float s = 2 * c < CHUNKS ? s0 : s1;
+    const uint64_t ss = f2(s, s);
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      acc[16 * c + j] =
+          f2_fma((static_cast<uint64_t>(r[c & 1][2 * j + 1]) << 32) | r[c & 1][2 * j], ss, acc[16 * c + j]);
+  }
+}
+
 // act(g) u, both activations in the form g / (1 + exp(-z)): z = g (SiLU), or
 // z = 2 sqrt(2 / pi) (g + 0.044715 g^3), since (1 + tanh(z / 2)) / 2 =
 // 1 / (1 + exp(-z)).  exp and the quotient are the fast f32 ones (a few ulp):
 // the 11-bit hardware tanh would show in the f32 scales of 8-bit rows.
 __device__ __forceinline__ float gate(float g, float u, int act) {
   const float z = act == WC_ACT_SILU ? g : 1.5957691216f * (g + 0.044715f * g * g * g);
-  return g * __frcp_rn(1.0f + __expf(-z)) * u;
+  return g * __fdividef(1.0f, 1.0f + __expf(-z)) * u;
 }
+
+__device__ __forceinline__ void regs_for_epilogue() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
+__device__ __forceinline__ void regs_given_back() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
+
+// After a wait ran out, the loads already issued still land in shared memory:
+// wait (again with a limit) for the last `stages` of the `issued` ones.
+__device__ __forceinline__ void drain_loads(uint64_t* full, uint32_t stages, uint32_t issued, uint32_t* status) {
+  for (uint32_t j = issued > stages ? issued - stages : 0; j < issued; ++j)
+    mbar_wait(&full[j % stages], (j / stages) & 1, status);
+}
+
+// ---------------------------------------------------------------- pairs of SMs
+
+// A cluster of two CTAs owns a 256 x 256 tile.  Each CTA loads its own 128
+// rows of A and the 128 weight rows of one column half; the even CTA's MMA
+// thread multiplies from both CTAs' shared memory into both CTAs' TMEM (each
+// its 128 rows x 256 columns).  Loads of both CTAs complete on the even CTA's
+// barriers, MMA completion is committed to both, and the epilogue warps of
+// both report to the even CTA that they have read a partial.
+namespace pair {
+
+constexpr int kBN = 256;
+constexpr int kStages = 6;
+constexpr int kStageBytes = kABytes + 128 * kFp8Block;
+constexpr int kOutBytes = 32 * 128;  // one warp's 32 rows x 32 f32 on the way out
+constexpr int kOffOut = kStages * kStageBytes;
+constexpr int kOffAmax = kOffOut + 8 * kOutBytes;
+constexpr int kOffBar = kOffAmax + 2 * kRows * 4;
+constexpr int kSmem = 1024 + kOffBar + 256;
+static_assert(kSmem <= 232448, "dynamic shared memory per block");
 
 template <bool GATED, typename OutT>
 __global__ void __launch_bounds__(kThreads, 1)
-    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+    fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                     const __grid_constant__ CUtensorMap tmU, const __grid_constant__ Fp8GemmParams p) {
   constexpr bool kCodes = sizeof(OutT) == 1;  // 8-bit rows out (gated)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBar);  // [kStages] operands landed
-  uint64_t* empty = full + kStages;                              // [kStages] MMA done with them
-  uint64_t* acc_full = empty + kStages;                          // [2] partial ready
-  uint64_t* acc_empty = acc_full + 2;                            // [2] partial read by the 8 epilogue warps
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBar);  // [kStages] even CTA: operands of both landed
+  uint64_t* empty = full + kStages;                              // [kStages] each CTA: MMA done with them
+  uint64_t* acc_full = empty + kStages;                          // [2] each CTA: partial ready
+  uint64_t* acc_empty = acc_full + 2;                            // [2] even CTA: partial read by 16 epilogue warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* status = p.status ? p.status : &g_fp8_status;
+  const uint32_t rank = cluster_rank();
 
   constexpr int kFeat = GATED ? kBN / 2 : kBN;  // output columns per tile
   const int kblocks = (p.k + kFp8Block - 1) / kFp8Block;
-  const int m_tiles = (p.m + kBM - 1) / kBM, n_tiles = (p.n + kFeat - 1) / kFeat;
+  const int m_tiles = (p.m + 2 * kRows - 1) / (2 * kRows), n_tiles = (p.n + kFeat - 1) / kFeat;
   const int64_t tiles = static_cast<int64_t>(m_tiles) * n_tiles;
+  const int64_t tile0 = cluster_id(), tile_step = num_clusters();
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -124,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 8);
+      mbar_init(&acc_empty[i], 16);
     }
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
@@ -132,110 +201,95 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (GATED) tma_prefetch_desc(&tmU);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, kTmemCols);
-    tmem_relinquish();
+    tmem_alloc_pair(tmem_slot, kTmemCols);
+    tmem_relinquish_pair();
   }
   tc_fence_before();
-  __syncthreads();
+  cluster_sync();  // barriers of both CTAs initialised, TMEM allocated
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();
   pdl_launch_next();
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    regs_given_back();
+    if (warp == 0 && lane == 0) {
       uint32_t i = 0;
       bool ok = true;
-      for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-        const int m0 = static_cast<int>(tile / n_tiles) * kBM, f0 = static_cast<int>(tile % n_tiles) * kFeat;
+      for (int64_t tile = tile0; tile < tiles && ok; tile += tile_step) {
+        const int m0 = static_cast<int>(tile / n_tiles) * 2 * kRows + static_cast<int>(rank) * kRows;
+        const int f0 = static_cast<int>(tile % n_tiles) * kFeat + static_cast<int>(rank) * (kFeat / 2);
         for (int kb = 0; kb < kblocks; ++kb, ++i) {
           const uint32_t s = i % kStages;
           if (!(ok = mbar_wait(&empty[s], ((i / kStages) & 1) ^ 1, status))) break;
-          mbar_arrive_expect_tx(&full[s], kStageBytes);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
           uint8_t* sa = smem + s * kStageBytes;
-          tma_load_2d(sa, &tmA, &full[s], kb * kFp8Block, m0);
-#pragma unroll
-          for (int c = 0; c < 4; ++c)  // 64 weight rows each
-            tma_load_2d(sa + kABytes + c * 64 * kFp8Block, GATED && (c & 1) ? &tmU : &tmW, &full[s], kb * kFp8Block,
-                        GATED ? f0 + (c >> 1) * 64 : f0 + c * 64);
+          const uint32_t bar = map_to_rank(&full[s], 0);
+          tma_load_2d_pair(sa, &tmA, bar, kb * kFp8Block, m0);
+          tma_load_2d_pair(sa + kABytes, &tmW, bar, kb * kFp8Block, f0);
+          tma_load_2d_pair(sa + kABytes + 64 * kFp8Block, GATED ? &tmU : &tmW, bar, kb * kFp8Block,
+                           GATED ? f0 : f0 + 64);
         }
       }
-      // After a timeout the loads already issued still land in this CTA's
-      // shared memory: wait for them before it exits.
-      if (!ok)
-        for (uint32_t j = i > kStages ? i - kStages : 0; j < i; ++j)
-          mbar_wait(&full[j % kStages], (j / kStages) & 1, status);
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_e4m3_f32(kBM, kBN);
+      // the odd CTA's loads complete on the even CTA's barriers; the cluster
+      // barrier at the end holds it until the even CTA has waited
+      if (!ok && rank == 0) drain_loads(full, kStages, i, status);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = idesc_e4m3_f32(2 * kRows, kBN);
       uint32_t i = 0;
       bool ok = true;
-      for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      for (int64_t tile = tile0; tile < tiles && ok; tile += tile_step) {
         for (int kb = 0; kb < kblocks; ++kb, ++i) {
           const uint32_t s = i % kStages, buf = i & 1;
-          ok = mbar_wait(&acc_empty[buf], ((i >> 1) & 1) ^ 1, status) &&
-               mbar_wait(&full[s], (i / kStages) & 1, status);
+          ok = mbar_wait_cluster(&acc_empty[buf], ((i >> 1) & 1) ^ 1, status) &&
+               mbar_wait_cluster(&full[s], (i / kStages) & 1, status);
           if (!ok) break;
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + s * kStageBytes);
-          const uint64_t adesc = sw128_kmajor_desc(sa), bdesc = sw128_kmajor_desc(sa + kABytes);
-#pragma unroll
-          for (int k = 0; k < kFp8Block / 32; ++k)
-            tc_mma_f8(tmem_base + buf * kBN, adesc + 2 * k, bdesc + 2 * k, idesc, k > 0 ? 1u : 0u);
-          tc_commit(&empty[s]);
-          tc_commit(&acc_full[buf]);
+          mma_block<true>(tmem_base + buf * kBN, sa, sa + kABytes, idesc);
+          tc_commit_pair(&empty[s]);
+          tc_commit_pair(&acc_full[buf]);
         }
       }
     }
-  } else if (warp >= 4) {
+  } else {
+    regs_for_epilogue();
     const int q = warp & 3, h = (warp >> 2) - 1;  // TMEM lane quarter, column half
-    uint8_t* stage = smem + kOffOut + (warp - 4) * kStageOutBytes;
+    uint8_t* stage = smem + kOffOut + (warp - 4) * kOutBytes;
     float* amax = reinterpret_cast<float*>(smem + kOffAmax);  // [half][row of the tile]
     const uint32_t tlane = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * 128;
+    const uint32_t empty0 = map_to_rank(&acc_empty[0], 0);
     uint32_t i = 0;
     bool ok = true;
-    for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-      const int m0 = static_cast<int>(tile / n_tiles) * kBM, f0 = static_cast<int>(tile % n_tiles) * kFeat;
+    for (int64_t tile = tile0; tile < tiles && ok; tile += tile_step) {
+      const int m0 = static_cast<int>(tile / n_tiles) * 2 * kRows + static_cast<int>(rank) * kRows;
+      const int f0 = static_cast<int>(tile % n_tiles) * kFeat;
       const int row = m0 + q * 32 + lane;
       const int nb = GATED ? f0 / kFp8Block : f0 / kFp8Block + h;  // block of weight rows
       const bool live = row < p.m && nb * kFp8Block < p.n;
       const float* sa = p.sa + row * p.ldsa;
       const float* sw = p.sw + nb * p.ldsw;
-      const float* sup = GATED ? p.sup + nb * p.ldsup : nullptr;
+      const float* sup = GATED ? p.sup + nb * p.ldsup : sw;
       uint64_t acc[64];  // 128 columns in pairs
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = 0ull;
+      float an = live ? __ldg(sa) : 0.f, wn = live ? __ldg(sw) : 0.f, un = GATED && live ? __ldg(sup) : 0.f;
       for (int kb = 0; kb < kblocks; ++kb, ++i) {
         const uint32_t buf = i & 1;
-        float s0 = 0.f, s1 = 0.f;
-        if (live) {
-          const float a = sa[kb];
-          s0 = a * sw[kb];
-          s1 = GATED ? a * sup[kb] : s0;
+        const float s0 = an * wn, s1 = GATED ? an * un : s0;
+        if (live && kb + 1 < kblocks) {  // the next block's scales arrive while this one is added
+          an = __ldg(sa + kb + 1);
+          wn = __ldg(sw + kb + 1);
+          if (GATED) un = __ldg(sup + kb + 1);
         }
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[buf], (i >> 1) & 1, status));
         if (!ok) break;
         tc_fence_after();
-        uint32_t r[2][32];
-        tmem_ld32_issue(tlane + buf * kBN, r[0]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_ld32_wait(r[c & 1]);
-          if (c < 3) {
-            tmem_ld32_issue(tlane + buf * kBN + 32 * (c + 1), r[(c + 1) & 1]);
-          } else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[buf]);
-          }
-          const float s = c < 2 ? s0 : s1;
-          const uint64_t ss = f2(s, s);
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            acc[16 * c + j] = f2_fma((static_cast<uint64_t>(r[c & 1][2 * j + 1]) << 32) | r[c & 1][2 * j], ss,
-                                     acc[16 * c + j]);
-        }
+        add_block<4>(tlane + buf * kBN, s0, s1, acc, [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(empty0 + buf * 8);
+        });
       }
       if (!ok) break;
 
@@ -244,17 +298,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 32; ++j)
           acc[j] = f2(gate(f2_lo(acc[j]), f2_lo(acc[32 + j]), p.act), gate(f2_hi(acc[j]), f2_hi(acc[32 + j]), p.act));
       }
-      const int col0 = f0 + h * (GATED ? 64 : 128);  // the thread's first output column
+      const int col0 = f0 + h * (kFeat / 2);  // the thread's first output column
       if constexpr (kCodes) {
         // The 64 results of this thread and those of the thread with the same
         // row in the other half are one block of 128.
         float a = 0.f;
 #pragma unroll
         for (int j = 0; j < 32; ++j) a = max_nan(a, max_nan(fabsf(f2_lo(acc[j])), fabsf(f2_hi(acc[j]))));
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // the tile before has read its maxima
-        amax[h * kBM + q * 32 + lane] = a;
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the maxima of the tile before have been read
+        amax[h * kRows + q * 32 + lane] = a;
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        const float sc = fp8_scale(max_nan(a, amax[(h ^ 1) * kBM + q * 32 + lane])), fac = fp8_factor(sc);
+        const float sc = fp8_scale(max_nan(a, amax[(h ^ 1) * kRows + q * 32 + lane])), fac = fp8_factor(sc);
         if (row < p.m) {
           if (h == 0) p.out_scales[row * p.ldos + nb] = sc;
           uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.ldo + col0;
@@ -292,10 +346,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint64_t lo = acc[16 * c + 2 * j], hi = acc[16 * c + 2 * j + 1];
-            *reinterpret_cast<ulonglong2*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_ulonglong2(lo, hi);
-          }
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<ulonglong2*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                make_ulonglong2(acc[16 * c + 2 * j], acc[16 * c + 2 * j + 1]);
           __syncwarp();
 #pragma unroll
           for (int t = 0; t < 8; ++t) {
@@ -315,12 +368,260 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   __syncwarp();
   tc_fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, kTmemCols);
+  }
+}
+
+}  // namespace pair
+
+// ---------------------------------------------------------------- single tiles
+
+// One 128 x BN tile per cluster of `split` CTAs, CTA r taking every split-th
+// block of K from r on.  The sums meet in shared memory: each CTA writes its
+// 128 x BN f32 over its operand stages, and after a cluster barrier CTA r
+// finishes rows r, r + split, ... adding the CTAs' values in rank order, one
+// warp per row (so a block of 128 results is one warp, and its maximum one
+// warp reduction).  Rows past m are neither loaded nor read back.
+namespace tile {
+
+template <int BN>
+struct Plan {
+  static constexpr int kStages = BN == 256 ? 4 : 6;
+  static constexpr int kStageBytes = kABytes + BN * kFp8Block;
+  static constexpr int kBufs = static_cast<int>(kTmemCols) / BN;
+  static constexpr int kOffBar = kStages * kStageBytes;
+  static constexpr int kSmem = 1024 + kOffBar + 256;
+  static_assert(kSmem <= 232448, "dynamic shared memory per block");
+  static_assert(kRows * BN * 4 <= kOffBar, "the sums fit over the operand stages");
+};
+
+// Byte offset of the 16-byte chunk c of row r of the sums (conflict-free both
+// for a thread per row and for a warp per row).
+template <int BN>
+__device__ __forceinline__ uint32_t sum_offset(int r, int c) {
+  return static_cast<uint32_t>(r * (BN * 4) + ((c ^ (r & 31)) << 4));
+}
+__device__ __forceinline__ float4 load_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+template <bool GATED, typename OutT, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+                    const __grid_constant__ CUtensorMap tmU, const __grid_constant__ Fp8GemmParams p, int split,
+                    int a_rows) {
+  using PL = Plan<BN>;
+  constexpr bool kCodes = sizeof(OutT) == 1;
+  constexpr int kChunks = BN / 64;  // 32-column chunks of a thread's half
+  static_assert(!GATED || BN == 256, "the gated product needs 128 features of both weights");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + PL::kOffBar);
+  uint64_t* empty = full + PL::kStages;
+  uint64_t* acc_full = empty + PL::kStages;
+  uint64_t* acc_empty = acc_full + PL::kBufs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + PL::kBufs);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t* status = p.status ? p.status : &g_fp8_status;
+
+  constexpr int kFeat = GATED ? BN / 2 : BN;
+  const int kblocks = (p.k + kFp8Block - 1) / kFp8Block;
+  const int n_tiles = (p.n + kFeat - 1) / kFeat;
+  const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int64_t tile = blockIdx.x / split;
+  const int m0 = static_cast<int>(tile / n_tiles) * kRows, f0 = static_cast<int>(tile % n_tiles) * kFeat;
+  const int rows = min(kRows, p.m - m0);
+  const int epi_warps = 2 * ((rows + 31) / 32);  // warps whose lanes hold rows of the matrix
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < PL::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < PL::kBufs; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], epi_warps);
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmW);
+    if (GATED) tma_prefetch_desc(&tmU);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+  pdl_launch_next();
+
+  if (warp < 4) {
+    regs_given_back();
+    if (warp == 0 && lane == 0) {
+      uint32_t i = 0;
+      bool ok = true;
+      for (int kb = rank; kb < kblocks; kb += split, ++i) {
+        const uint32_t s = i % PL::kStages;
+        if (!(ok = mbar_wait(&empty[s], ((i / PL::kStages) & 1) ^ 1, status))) break;
+        mbar_arrive_expect_tx(&full[s], a_rows * kFp8Block + BN * kFp8Block);
+        uint8_t* sa = smem + s * PL::kStageBytes;
+        tma_load_2d(sa, &tmA, &full[s], kb * kFp8Block, m0);
+#pragma unroll
+        for (int c = 0; c < BN / 64; ++c)  // 64 weight rows each
+          tma_load_2d(sa + kABytes + c * 64 * kFp8Block, GATED && (c & 1) ? &tmU : &tmW, &full[s], kb * kFp8Block,
+                      GATED ? f0 + (c >> 1) * 64 : f0 + c * 64);
+      }
+      if (!ok) drain_loads(full, PL::kStages, i, status);
+    } else if (warp == 1 && lane == 0) {
+      constexpr uint32_t idesc = idesc_e4m3_f32(kRows, BN);
+      uint32_t i = 0;
+      for (int kb = rank; kb < kblocks; kb += split, ++i) {
+        const uint32_t s = i % PL::kStages, buf = i % PL::kBufs;
+        if (!mbar_wait(&acc_empty[buf], ((i / PL::kBufs) & 1) ^ 1, status) ||
+            !mbar_wait(&full[s], (i / PL::kStages) & 1, status))
+          break;
+        tc_fence_after();
+        const uint32_t sa = smem_u32(smem + s * PL::kStageBytes);
+        mma_block<false>(tmem_base + buf * BN, sa, sa + kABytes, idesc);
+        tc_commit(&empty[s]);
+        tc_commit(&acc_full[buf]);
+      }
+    }
+  } else {
+    regs_for_epilogue();
+    const int q = warp & 3, h = (warp >> 2) - 1;
+    if (q * 32 < rows) {
+      const uint32_t tlane = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * (BN / 2);
+      const int lrow = q * 32 + lane, row = m0 + lrow;
+      const int nb = f0 / kFp8Block + (GATED || BN == 128 ? 0 : h);  // block of weight rows
+      const bool live = lrow < rows && nb * kFp8Block < p.n;
+      const float* sa = p.sa + row * p.ldsa;
+      const float* sw = p.sw + nb * p.ldsw;
+      const float* sup = GATED ? p.sup + nb * p.ldsup : sw;
+      uint64_t acc[16 * kChunks];
+#pragma unroll
+      for (int j = 0; j < 16 * kChunks; ++j) acc[j] = 0ull;
+      const bool any = live && rank < kblocks;
+      float an = any ? __ldg(sa + rank) : 0.f, wn = any ? __ldg(sw + rank) : 0.f,
+            un = GATED && any ? __ldg(sup + rank) : 0.f;
+      uint32_t i = 0;
+      for (int kb = rank; kb < kblocks; kb += split, ++i) {
+        const uint32_t buf = i % PL::kBufs;
+        const float s0 = an * wn, s1 = GATED ? an * un : s0;
+        if (live && kb + split < kblocks) {
+          an = __ldg(sa + kb + split);
+          wn = __ldg(sw + kb + split);
+          if (GATED) un = __ldg(sup + kb + split);
+        }
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[buf], (i / PL::kBufs) & 1, status))) break;
+        tc_fence_after();
+        add_block<kChunks>(tlane + buf * BN, s0, s1, acc, [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        });
+      }
+      // The last partial was committed after every MMA of this CTA, so the
+      // operand stages are free for the sums.
+#pragma unroll
+      for (int j = 0; j < 8 * kChunks; ++j)
+        *reinterpret_cast<ulonglong2*>(smem + sum_offset<BN>(lrow, h * (BN / 8) + j)) =
+            make_ulonglong2(acc[2 * j], acc[2 * j + 1]);
+    }
+  }
+
+  __syncwarp();
+  if (split > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+
+  if (warp >= 4) {
+    const uint32_t base = smem_u32(smem);
+    // the sum over the cluster of chunk c of row r
+    auto total = [&](int r, int c) {
+      const uint32_t at = base + sum_offset<BN>(r, c);
+      if (split == 1) {
+        float4 v;
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                     : "r"(at)
+                     : "memory");
+        return v;
+      }
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int s = 0; s < split; ++s) {
+        uint32_t remote;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(s));
+        const float4 u = load_cluster(remote);
+        v.x += u.x;
+        v.y += u.y;
+        v.z += u.z;
+        v.w += u.w;
+      }
+      return v;
+    };
+    for (int r = rank + split * (warp - 4); r < rows; r += split * 8) {
+      const int64_t row = m0 + r;
+      if constexpr (GATED) {
+        // lane: features 4 lane .. 4 lane + 3 of the tile's 128
+        const int c = (lane >> 4) * 32 + (lane & 15);
+        const float4 g = total(r, c), u = total(r, c + 16);
+        const float4 v = make_float4(gate(g.x, u.x, p.act), gate(g.y, u.y, p.act), gate(g.z, u.z, p.act),
+                                     gate(g.w, u.w, p.act));
+        const int col = f0 + lane * 4;
+        if constexpr (kCodes) {
+          const float a = max_nan(max_nan(fabsf(v.x), fabsf(v.y)), max_nan(fabsf(v.z), fabsf(v.w)));
+          const float sc = fp8_scale(warp_max_nan(a)), fac = fp8_factor(sc);
+          if (lane == 0) p.out_scales[row * p.ldos + f0 / kFp8Block] = sc;
+          store_codes4(static_cast<uint8_t*>(p.out) + row * p.ldo + col, p.n - col,
+                       pack_e4m3x4(v.x * fac, v.y * fac, v.z * fac, v.w * fac));
+        } else {
+          store4(static_cast<OutT*>(p.out) + row * p.ldo + col, p.n - col, p.vec_o, v);
+        }
+      } else {
+        const OutT* res = static_cast<const OutT*>(p.residual);
+#pragma unroll
+        for (int c = 0; c < BN / 128; ++c) {
+          const int col = f0 + c * 128 + lane * 4;
+          float4 rv = res ? load4(res + row * p.ldr + col, p.n - col, p.vec_r) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 v = total(r, c * 32 + lane);
+          rv.x += v.x;
+          rv.y += v.y;
+          rv.z += v.z;
+          rv.w += v.w;
+          store4(static_cast<OutT*>(p.out) + row * p.ldo + col, p.n - col, p.vec_o, rv);
+        }
+      }
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  if (split > 1)
+    cluster_sync();  // no CTA leaves while another reads its sums
+  else
+    __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, kTmemCols);
   }
 }
+
+}  // namespace tile
+
+// ---------------------------------------------------------------- host
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -353,26 +654,82 @@ bool codes_map(CUtensorMap* m, const uint8_t* ptr, int64_t rows, int64_t k, int6
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool GATED, typename OutT>
-cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
-  static bool attr_set[64] = {};
+// Largest dynamic shared memory, once per device and kernel.
+template <auto KERNEL>
+cudaError_t allow_smem(int bytes) {
+  static bool set[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!attr_set[dev]) {
-    e = cudaFuncSetAttribute(fp8_gemm_kernel<GATED, OutT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (!set[dev]) {
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
-    attr_set[dev] = true;
+    set[dev] = true;
   }
+  return cudaSuccess;
+}
+
+cudaLaunchAttribute cluster_of(int n) {
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeClusterDimension;
+  a.val.clusterDim.x = n;
+  a.val.clusterDim.y = 1;
+  a.val.clusterDim.z = 1;
+  return a;
+}
+
+template <bool GATED, typename OutT>
+cudaError_t launch_pair(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
+  constexpr auto kernel = pair::fp8_pair_kernel<GATED, OutT>;
+  cudaError_t e = allow_smem<kernel>(pair::kSmem);
+  if (e != cudaSuccess) return e;
   CUtensorMap ta, tw, tu;
-  if (!codes_map(&ta, p.a, p.m, p.k, p.lda, kBM) || !codes_map(&tw, p.w, p.n, p.k, p.ldw, 64) ||
+  if (!codes_map(&ta, p.a, p.m, p.k, p.lda, kRows) || !codes_map(&tw, p.w, p.n, p.k, p.ldw, 64) ||
       !codes_map(&tu, GATED ? p.up : p.w, p.n, p.k, GATED ? p.ldup : p.ldw, 64))
     return cudaErrorInvalidValue;
-  constexpr int kFeat = GATED ? kBN / 2 : kBN;
-  const int64_t tiles = static_cast<int64_t>((p.m + kBM - 1) / kBM) * ((p.n + kFeat - 1) / kFeat);
-  const int grid = static_cast<int>(std::min<int64_t>(tiles, num_sms));
-  return launch_pdl(fp8_gemm_kernel<GATED, OutT>, dim3(grid), dim3(kThreads), kSmem, st, nullptr, 0, ta, tw, tu, p);
+  constexpr int kFeat = GATED ? pair::kBN / 2 : pair::kBN;
+  const int64_t tiles = static_cast<int64_t>((p.m + 2 * kRows - 1) / (2 * kRows)) * ((p.n + kFeat - 1) / kFeat);
+  const int clusters = static_cast<int>(std::min<int64_t>(tiles, std::max(1, num_sms / 2)));
+  const cudaLaunchAttribute attr = cluster_of(2);
+  return launch_pdl(kernel, dim3(2 * clusters), dim3(kThreads), pair::kSmem, st, &attr, 1, ta, tw, tu, p);
+}
+
+template <bool GATED, typename OutT, int BN>
+cudaError_t launch_tile(const Fp8GemmParams& p, int split, cudaStream_t st) {
+  constexpr auto kernel = tile::fp8_tile_kernel<GATED, OutT, BN>;
+  cudaError_t e = allow_smem<kernel>(tile::Plan<BN>::kSmem);
+  if (e != cudaSuccess) return e;
+  // rows of a box of A: as many as there are, in steps of the swizzle's eight
+  const int a_rows = std::min(kRows, (p.m + 7) / 8 * 8);
+  CUtensorMap ta, tw, tu;
+  if (!codes_map(&ta, p.a, p.m, p.k, p.lda, a_rows) || !codes_map(&tw, p.w, p.n, p.k, p.ldw, 64) ||
+      !codes_map(&tu, GATED ? p.up : p.w, p.n, p.k, GATED ? p.ldup : p.ldw, 64))
+    return cudaErrorInvalidValue;
+  constexpr int kFeat = GATED ? BN / 2 : BN;
+  const int64_t tiles = static_cast<int64_t>((p.m + kRows - 1) / kRows) * ((p.n + kFeat - 1) / kFeat);
+  if (tiles * split > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  const cudaLaunchAttribute attr = cluster_of(split);
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * split)), dim3(kThreads), tile::Plan<BN>::kSmem, st,
+                    &attr, split > 1 ? 1 : 0, ta, tw, tu, p, split, a_rows);
+}
+
+template <bool GATED, typename OutT>
+cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
+  constexpr int BN = GATED ? 256 : 128;
+  constexpr int kFeat = 128;  // output columns of a single tile
+  const int64_t kblocks = (static_cast<int64_t>(p.k) + kFp8Block - 1) / kFp8Block;
+  const int64_t tiles = static_cast<int64_t>((p.m + kRows - 1) / kRows) * ((p.n + kFeat - 1) / kFeat);
+  if (tiles > 2 * num_sms) return launch_pair<GATED, OutT>(p, num_sms, st);
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= num_sms && split * 2 <= kblocks) split *= 2;
+#ifdef WC_FP8_SWEEP
+  if (const char* f = getenv("WC_FP8_FORCE")) {
+    if (atoi(f) == 0) return launch_pair<GATED, OutT>(p, num_sms, st);
+    split = atoi(f);
+  }
+#endif
+  return launch_tile<GATED, OutT, BN>(p, split, st);
 }
 
 }  // namespace
