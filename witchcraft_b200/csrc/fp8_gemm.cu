@@ -241,8 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int64_t tile = tile0; tile < tiles && ok; tile += tile_step) {
         for (int kb = 0; kb < kblocks; ++kb, ++i) {
           const uint32_t s = i % kStages, buf = i & 1;
-          ok = mbar_wait_cluster(&acc_empty[buf], ((i >> 1) & 1) ^ 1, status) &&
-               mbar_wait_cluster(&full[s], (i / kStages) & 1, status);
+          ok = mbar_wait(&acc_empty[buf], ((i >> 1) & 1) ^ 1, status) &&
+               mbar_wait(&full[s], (i / kStages) & 1, status);
           if (!ok) break;
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + s * kStageBytes);
