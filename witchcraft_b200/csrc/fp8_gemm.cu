@@ -6,8 +6,8 @@
 // The scales change with every block of 128 columns, so the tensor core's
 // accumulator cannot run over the whole of K: each block's P_b goes to one of
 // a few TMEM buffers, and the epilogue warps add scale * P_b to sums that they
-// keep in registers (one multiply-add per element and block, packed in pairs)
-// while the tensor core fills the next buffer.  A thread of the epilogue owns
+// keep in registers (one multiply-add per element and block) while the tensor
+// core fills the next buffer.  A thread of the epilogue owns
 // one row (a TMEM lane) and half of the tile's columns, so its row scale is
 // one register and the weight scale of its columns one value per block.
 // For the gated product the 256 columns of a tile are 64 gate features, the
@@ -103,10 +103,13 @@ __device__ __forceinline__ void tmem_ld32_wait(uint32_t (&r)[32]) {
                : "memory");
 }
 
-// acc[] (column pairs) += s0 * (first half) or s1 * (second half) of the
-// 32 CHUNKS columns at taddr; calls `read` once all of them are in registers.
+// acc[] += s0 * (first half) or s1 * (second half) of the 32 CHUNKS columns at
+// taddr; calls `read` once all of them are in registers.  Scalar
+// multiply-adds: the packed form needs register pairs that the TMEM load's
+// results have to be moved into, which cost more than it saved (8192 x 4096 x
+// 8192: 374 us packed, 353 us scalar).
 template <int CHUNKS, typename Read>
-__device__ __forceinline__ void add_block(uint32_t taddr, float s0, float s1, uint64_t (&acc)[16 * CHUNKS], Read read) {
+__device__ __forceinline__ void add_block(uint32_t taddr, float s0, float s1, float (&acc)[32 * CHUNKS], Read read) {
   uint32_t r[2][32];
   tmem_ld32_issue(taddr, r[0]);
 #pragma unroll
@@ -117,11 +120,30 @@ __device__ __forceinline__ void add_block(uint32_t taddr, float s0, float s1, ui
     else
       read();
     const float s = 2 * c < CHUNKS ? s0 : s1;
-    const uint64_t ss = f2(s, s);
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      acc[16 * c + j] =
-          f2_fma((static_cast<uint64_t>(r[c & 1][2 * j + 1]) << 32) | r[c & 1][2 * j], ss, acc[16 * c + j]);
+    for (int j = 0; j < 32; ++j) acc[32 * c + j] = __fmaf_rn(__uint_as_float(r[c & 1][j]), s, acc[32 * c + j]);
+  }
+}
+
+// The scales of one thread's row and columns, block by block, two blocks
+// ahead of their use: a load from L2 takes about as long as a block.  The
+// loads are volatile, or the compiler moves them down to their use.
+struct Scales {
+  const float *a, *w, *u;  // the row's, the columns', the up columns'
+  bool live;
+  float va[2], vw[2], vu[2];
+};
+__device__ __forceinline__ float load_ahead(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+template <bool GATED>
+__device__ __forceinline__ void fetch_scales(Scales& s, int slot, int kb, int kblocks) {
+  if (s.live && kb < kblocks) {
+    s.va[slot] = load_ahead(s.a + kb);
+    s.vw[slot] = load_ahead(s.w + kb);
+    if (GATED) s.vu[slot] = load_ahead(s.u + kb);
   }
 }
 
@@ -172,9 +194,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBar);  // [kStages] even CTA: operands of both landed
-  uint64_t* empty = full + kStages;                              // [kStages] each CTA: MMA done with them
-  uint64_t* acc_full = empty + kStages;                          // [2] each CTA: partial ready
-  uint64_t* acc_empty = acc_full + 2;                            // [2] even CTA: partial read by 16 epilogue warps
+  uint64_t* done = full + kStages;       // [kStages] each CTA: MMA done (stage free, partial ready)
+  uint64_t* acc_empty = done + kStages;  // [2] even CTA: partial read by 16 epilogue warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* status = p.status ? p.status : &g_fp8_status;
@@ -189,12 +210,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&done[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 16);
-    }
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_empty[i], 16);
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmW);
@@ -221,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int f0 = static_cast<int>(tile % n_tiles) * kFeat + static_cast<int>(rank) * (kFeat / 2);
         for (int kb = 0; kb < kblocks; ++kb, ++i) {
           const uint32_t s = i % kStages;
-          if (!(ok = mbar_wait(&empty[s], ((i / kStages) & 1) ^ 1, status))) break;
+          if (!(ok = mbar_wait(&done[s], ((i / kStages) & 1) ^ 1, status))) break;
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
           uint8_t* sa = smem + s * kStageBytes;
           const uint32_t bar = map_to_rank(&full[s], 0);
@@ -241,14 +259,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int64_t tile = tile0; tile < tiles && ok; tile += tile_step) {
         for (int kb = 0; kb < kblocks; ++kb, ++i) {
           const uint32_t s = i % kStages, buf = i & 1;
-          ok = mbar_wait(&acc_empty[buf], ((i >> 1) & 1) ^ 1, status) &&
-               mbar_wait(&full[s], (i / kStages) & 1, status);
+          ok = mbar_wait(&full[s], (i / kStages) & 1, status) &&
+               mbar_wait(&acc_empty[buf], ((i >> 1) & 1) ^ 1, status);
           if (!ok) break;
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + s * kStageBytes);
           mma_block<true>(tmem_base + buf * kBN, sa, sa + kABytes, idesc);
-          tc_commit_pair(&empty[s]);
-          tc_commit_pair(&acc_full[buf]);
+          tc_commit_pair(&done[s]);
         }
       }
     }
@@ -259,44 +276,58 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* amax = reinterpret_cast<float*>(smem + kOffAmax);  // [half][row of the tile]
     const uint32_t tlane = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * 128;
     const uint32_t empty0 = map_to_rank(&acc_empty[0], 0);
+    Scales sc{};
+    auto open_tile = [&](int64_t tile) {  // its scales' addresses and first two blocks
+      const int row = static_cast<int>(tile / n_tiles) * 2 * kRows + static_cast<int>(rank) * kRows + q * 32 + lane;
+      const int f0 = static_cast<int>(tile % n_tiles) * kFeat;
+      const int nb = GATED ? f0 / kFp8Block : f0 / kFp8Block + h;  // block of weight rows
+      sc.live = tile < tiles && row < p.m && nb * kFp8Block < p.n;
+      sc.a = p.sa + row * p.ldsa;
+      sc.w = p.sw + nb * p.ldsw;
+      if (GATED) sc.u = p.sup + nb * p.ldsup;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        sc.va[j] = sc.vw[j] = sc.vu[j] = 0.f;
+        fetch_scales<GATED>(sc, j, j, kblocks);
+      }
+    };
     uint32_t i = 0;
     bool ok = true;
+    open_tile(tile0);
     for (int64_t tile = tile0; tile < tiles && ok; tile += tile_step) {
       const int m0 = static_cast<int>(tile / n_tiles) * 2 * kRows + static_cast<int>(rank) * kRows;
       const int f0 = static_cast<int>(tile % n_tiles) * kFeat;
-      const int row = m0 + q * 32 + lane;
-      const int nb = GATED ? f0 / kFp8Block : f0 / kFp8Block + h;  // block of weight rows
-      const bool live = row < p.m && nb * kFp8Block < p.n;
-      const float* sa = p.sa + row * p.ldsa;
-      const float* sw = p.sw + nb * p.ldsw;
-      const float* sup = GATED ? p.sup + nb * p.ldsup : sw;
-      uint64_t acc[64];  // 128 columns in pairs
+      float acc[128];
 #pragma unroll
-      for (int j = 0; j < 64; ++j) acc[j] = 0ull;
-      float an = live ? __ldg(sa) : 0.f, wn = live ? __ldg(sw) : 0.f, un = GATED && live ? __ldg(sup) : 0.f;
-      for (int kb = 0; kb < kblocks; ++kb, ++i) {
-        const uint32_t buf = i & 1;
-        const float s0 = an * wn, s1 = GATED ? an * un : s0;
-        if (live && kb + 1 < kblocks) {  // the next block's scales arrive while this one is added
-          an = __ldg(sa + kb + 1);
-          wn = __ldg(sw + kb + 1);
-          if (GATED) un = __ldg(sup + kb + 1);
+      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+      for (int kb0 = 0; kb0 < kblocks && ok; kb0 += 2) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int kb = kb0 + j;
+          if (kb < kblocks && ok) {
+            const uint32_t buf = i & 1, st = i % kStages;
+            const float s0 = sc.va[j] * sc.vw[j], s1 = GATED ? sc.va[j] * sc.vu[j] : s0;
+            fetch_scales<GATED>(sc, j, kb + 2, kblocks);
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&done[st], (i / kStages) & 1, status));
+            if (ok) {
+              tc_fence_after();
+              add_block<4>(tlane + buf * kBN, s0, s1, acc, [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_remote(empty0 + buf * 8);
+              });
+            }
+            ++i;
+          }
         }
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[buf], (i >> 1) & 1, status));
-        if (!ok) break;
-        tc_fence_after();
-        add_block<4>(tlane + buf * kBN, s0, s1, acc, [&] {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_remote(empty0 + buf * 8);
-        });
       }
       if (!ok) break;
+      open_tile(tile + tile_step);  // arrives while this tile is written
 
+      const int row = m0 + q * 32 + lane;
       if constexpr (GATED) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          acc[j] = f2(gate(f2_lo(acc[j]), f2_lo(acc[32 + j]), p.act), gate(f2_hi(acc[j]), f2_hi(acc[32 + j]), p.act));
+        for (int j = 0; j < 64; ++j) acc[j] = gate(acc[j], acc[64 + j], p.act);
       }
       const int col0 = f0 + h * (kFeat / 2);  // the thread's first output column
       if constexpr (kCodes) {
@@ -304,21 +335,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         // row in the other half are one block of 128.
         float a = 0.f;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) a = max_nan(a, max_nan(fabsf(f2_lo(acc[j])), fabsf(f2_hi(acc[j]))));
+        for (int j = 0; j < 64; ++j) a = max_nan(a, fabsf(acc[j]));
         asm volatile("bar.sync 1, 256;" ::: "memory");  // the maxima of the tile before have been read
         amax[h * kRows + q * 32 + lane] = a;
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        const float sc = fp8_scale(max_nan(a, amax[(h ^ 1) * kRows + q * 32 + lane])), fac = fp8_factor(sc);
+        const float os = fp8_scale(max_nan(a, amax[(h ^ 1) * kRows + q * 32 + lane])), fac = fp8_factor(os);
         if (row < p.m) {
-          if (h == 0) p.out_scales[row * p.ldos + nb] = sc;
+          if (h == 0) p.out_scales[row * p.ldos + f0 / kFp8Block] = os;
           uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.ldo + col0;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {  // 16 codes
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              w[e] = pack_e4m3x4(f2_lo(acc[8 * c + 2 * e]) * fac, f2_hi(acc[8 * c + 2 * e]) * fac,
-                                 f2_lo(acc[8 * c + 2 * e + 1]) * fac, f2_hi(acc[8 * c + 2 * e + 1]) * fac);
+              w[e] = pack_e4m3x4(acc[16 * c + 4 * e] * fac, acc[16 * c + 4 * e + 1] * fac, acc[16 * c + 4 * e + 2] * fac,
+                                 acc[16 * c + 4 * e + 3] * fac);
             const int left = p.n - col0 - 16 * c;
             if (left >= 16) {
               *reinterpret_cast<uint4*>(o + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -347,8 +378,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<ulonglong2*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                make_ulonglong2(acc[16 * c + 2 * j], acc[16 * c + 2 * j + 1]);
+            *reinterpret_cast<float4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                make_float4(acc[32 * c + 4 * j], acc[32 * c + 4 * j + 1], acc[32 * c + 4 * j + 2], acc[32 * c + 4 * j + 3]);
           __syncwarp();
 #pragma unroll
           for (int t = 0; t < 8; ++t) {
@@ -425,9 +456,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + PL::kOffBar);
-  uint64_t* empty = full + PL::kStages;
-  uint64_t* acc_full = empty + PL::kStages;
-  uint64_t* acc_empty = acc_full + PL::kBufs;
+  uint64_t* done = full + PL::kStages;  // MMA done: stage free, partial ready
+  uint64_t* acc_empty = done + PL::kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + PL::kBufs);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* status = p.status ? p.status : &g_fp8_status;
@@ -444,12 +474,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < PL::kStages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&done[i], 1);
     }
-    for (int i = 0; i < PL::kBufs; ++i) {
-      mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], epi_warps);
-    }
+    for (int i = 0; i < PL::kBufs; ++i) mbar_init(&acc_empty[i], epi_warps);
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmW);
@@ -473,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int kb = rank; kb < kblocks; kb += split, ++i) {
         const uint32_t s = i % PL::kStages;
-        if (!(ok = mbar_wait(&empty[s], ((i / PL::kStages) & 1) ^ 1, status))) break;
+        if (!(ok = mbar_wait(&done[s], ((i / PL::kStages) & 1) ^ 1, status))) break;
         mbar_arrive_expect_tx(&full[s], a_rows * kFp8Block + BN * kFp8Block);
         uint8_t* sa = smem + s * PL::kStageBytes;
         tma_load_2d(sa, &tmA, &full[s], kb * kFp8Block, m0);
@@ -488,14 +515,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t i = 0;
       for (int kb = rank; kb < kblocks; kb += split, ++i) {
         const uint32_t s = i % PL::kStages, buf = i % PL::kBufs;
-        if (!mbar_wait(&acc_empty[buf], ((i / PL::kBufs) & 1) ^ 1, status) ||
-            !mbar_wait(&full[s], (i / PL::kStages) & 1, status))
+        if (!mbar_wait(&full[s], (i / PL::kStages) & 1, status) ||
+            !mbar_wait(&acc_empty[buf], ((i / PL::kBufs) & 1) ^ 1, status))
           break;
         tc_fence_after();
         const uint32_t sa = smem_u32(smem + s * PL::kStageBytes);
         mma_block<false>(tmem_base + buf * BN, sa, sa + kABytes, idesc);
-        tc_commit(&empty[s]);
-        tc_commit(&acc_full[buf]);
+        tc_commit(&done[s]);
       }
     }
   } else {
@@ -505,39 +531,45 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t tlane = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * (BN / 2);
       const int lrow = q * 32 + lane, row = m0 + lrow;
       const int nb = f0 / kFp8Block + (GATED || BN == 128 ? 0 : h);  // block of weight rows
-      const bool live = lrow < rows && nb * kFp8Block < p.n;
-      const float* sa = p.sa + row * p.ldsa;
-      const float* sw = p.sw + nb * p.ldsw;
-      const float* sup = GATED ? p.sup + nb * p.ldsup : sw;
-      uint64_t acc[16 * kChunks];
+      Scales sc{};
+      sc.live = lrow < rows && nb * kFp8Block < p.n;
+      sc.a = p.sa + row * p.ldsa;
+      sc.w = p.sw + nb * p.ldsw;
+      if (GATED) sc.u = p.sup + nb * p.ldsup;
 #pragma unroll
-      for (int j = 0; j < 16 * kChunks; ++j) acc[j] = 0ull;
-      const bool any = live && rank < kblocks;
-      float an = any ? __ldg(sa + rank) : 0.f, wn = any ? __ldg(sw + rank) : 0.f,
-            un = GATED && any ? __ldg(sup + rank) : 0.f;
+      for (int j = 0; j < 2; ++j) fetch_scales<GATED>(sc, j, rank + j * split, kblocks);
+      float acc[32 * kChunks];
+#pragma unroll
+      for (int j = 0; j < 32 * kChunks; ++j) acc[j] = 0.f;
       uint32_t i = 0;
-      for (int kb = rank; kb < kblocks; kb += split, ++i) {
-        const uint32_t buf = i % PL::kBufs;
-        const float s0 = an * wn, s1 = GATED ? an * un : s0;
-        if (live && kb + split < kblocks) {
-          an = __ldg(sa + kb + split);
-          wn = __ldg(sw + kb + split);
-          if (GATED) un = __ldg(sup + kb + split);
+      bool ok = true;
+      for (int kb0 = rank; kb0 < kblocks && ok; kb0 += 2 * split) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int kb = kb0 + j * split;
+          if (kb < kblocks && ok) {
+            const uint32_t buf = i % PL::kBufs, st = i % PL::kStages;
+            const float s0 = sc.va[j] * sc.vw[j], s1 = GATED ? sc.va[j] * sc.vu[j] : s0;
+            fetch_scales<GATED>(sc, j, kb + 2 * split, kblocks);
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&done[st], (i / PL::kStages) & 1, status));
+            if (ok) {
+              tc_fence_after();
+              add_block<kChunks>(tlane + buf * BN, s0, s1, acc, [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&acc_empty[buf]);
+              });
+            }
+            ++i;
+          }
         }
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[buf], (i / PL::kBufs) & 1, status))) break;
-        tc_fence_after();
-        add_block<kChunks>(tlane + buf * BN, s0, s1, acc, [&] {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[buf]);
-        });
       }
       // The last partial was committed after every MMA of this CTA, so the
       // operand stages are free for the sums.
 #pragma unroll
       for (int j = 0; j < 8 * kChunks; ++j)
-        *reinterpret_cast<ulonglong2*>(smem + sum_offset<BN>(lrow, h * (BN / 8) + j)) =
-            make_ulonglong2(acc[2 * j], acc[2 * j + 1]);
+        *reinterpret_cast<float4*>(smem + sum_offset<BN>(lrow, h * (BN / 8) + j)) =
+            make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
     }
   }
 
