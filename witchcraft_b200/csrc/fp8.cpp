@@ -193,6 +193,8 @@ extern "C" int wc_fp8_matmul(const void* d_a, int64_t lda, const float* d_sa, in
   p.ldo = ldo;
   p.vec_o = vec4(d_out, ldo, out_type);
   p.vec_r = d_residual && vec4(d_residual, ldr, out_type);
+  p.box_o = aligned(d_out, ldo, 16, out_type);
+  p.box_r = d_residual && aligned(d_residual, ldr, 16, out_type);
   return done(fp8_gemm_launch(false, out_type, p, sms, static_cast<cudaStream_t>(stream)), "product launch");
 }
 
@@ -225,6 +227,7 @@ extern "C" int wc_fp8_gated_matmul(const void* d_a, int64_t lda, const float* d_
   p.out_scales = d_out_scales;
   p.ldos = ldos;
   p.vec_o = vec4(d_out, ldo, out_type);
+  p.box_o = aligned(d_out, ldo, 16, out_type);
   return done(fp8_gemm_launch(true, out_type, p, sms, static_cast<cudaStream_t>(stream)), "gated product launch");
 }
 

@@ -70,13 +70,42 @@ __device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint6
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// One block of 128 columns: four MMAs of 32.
-template <bool PAIR>
-__device__ __forceinline__ void mma_block(uint32_t d_tmem, uint32_t a_smem, uint32_t b_smem, uint32_t idesc) {
-  const uint64_t adesc = sw128_kmajor_desc(a_smem), bdesc = sw128_kmajor_desc(b_smem);
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// The MMA warp's loop over `steps` blocks: STAGES operand stages of
+// STAGE_BYTES (A, then B) and two partials of BN columns.  The whole warp
+// runs it and one lane issues, so that descriptors stay in uniform registers:
+// the warp shares its scheduler with two epilogue warps that are busy with
+// multiply-adds, and every instruction in this loop is slow.
+template <bool PAIR, int STAGES, int STAGE_BYTES, int BN, typename Commit>
+__device__ __forceinline__ void mma_loop(uint32_t tmem, uint32_t idesc, uint32_t smem, uint64_t* full, uint64_t* done,
+                                         uint64_t* acc_empty, uint32_t steps, uint32_t* status, Commit commit) {
+  const uint64_t a0 = sw128_kmajor_desc(smem), b0 = sw128_kmajor_desc(smem + kABytes);
+  uint32_t s = 0, round = 0;
+#pragma unroll 1
+  for (uint32_t i = 0; i < steps; ++i) {
+    const uint32_t buf = i & 1;
+    const bool ok = mbar_wait(&full[s], round & 1, status) && mbar_wait(&acc_empty[buf], ((i >> 1) & 1) ^ 1, status);
+    if (!__all_sync(0xFFFFFFFFu, ok)) return;  // one way out for the whole warp
+    tc_fence_after();
+    const uint64_t a = a0 + s * (STAGE_BYTES >> 4), b = b0 + s * (STAGE_BYTES >> 4);
+    const uint32_t d = tmem + buf * BN;
+    if (elect_one()) {
 #pragma unroll
-  for (int k = 0; k < kFp8Block / 32; ++k)
-    tc_mma_f8<PAIR>(d_tmem, adesc + 2 * k, bdesc + 2 * k, idesc, k > 0 ? 1u : 0u);
+      for (int k = 0; k < kFp8Block / 32; ++k) tc_mma_f8<PAIR>(d, a + 2 * k, b + 2 * k, idesc, k > 0 ? 1u : 0u);
+      commit(&done[s]);
+    }
+    __syncwarp();
+    if (++s == STAGES) {
+      s = 0;
+      ++round;
+    }
+  }
 }
 
 // 32 lanes x 32 columns of f32: issue, and wait for everything issued.  The
@@ -111,17 +140,22 @@ __device__ __forceinline__ void tmem_ld32_wait(uint32_t (&r)[32]) {
 template <int CHUNKS, typename Read>
 __device__ __forceinline__ void add_block(uint32_t taddr, float s0, float s1, float (&acc)[32 * CHUNKS], Read read) {
   uint32_t r[2][32];
-  tmem_ld32_issue(taddr, r[0]);
-#pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    tmem_ld32_wait(r[c & 1]);
-    if (c + 1 < CHUNKS)
-      tmem_ld32_issue(taddr + 32 * (c + 1), r[(c + 1) & 1]);
-    else
-      read();
+  auto fma = [&](int c) {
     const float s = 2 * c < CHUNKS ? s0 : s1;
 #pragma unroll
     for (int j = 0; j < 32; ++j) acc[32 * c + j] = __fmaf_rn(__uint_as_float(r[c & 1][j]), s, acc[32 * c + j]);
+  };
+  tmem_ld32_issue(taddr, r[0]);
+  tmem_ld32_issue(taddr + 32, r[1]);
+#pragma unroll
+  for (int c = 0; c < CHUNKS; c += 2) {
+    tmem_ld32_wait(r[0]);
+    tmem_ld32_wait(r[1]);
+    if (c + 2 >= CHUNKS) read();
+    fma(c);
+    if (c + 2 < CHUNKS) tmem_ld32_issue(taddr + 32 * (c + 2), r[0]);
+    fma(c + 1);
+    if (c + 2 < CHUNKS) tmem_ld32_issue(taddr + 32 * (c + 3), r[1]);
   }
 }
 
@@ -166,6 +200,38 @@ __device__ __forceinline__ void drain_loads(uint64_t* full, uint32_t stages, uin
     mbar_wait(&full[j % stages], (j / stages) & 1, status);
 }
 
+// 16 bytes of a row of results: from f32, and added to f32.
+template <typename T>
+struct Pack;
+template <>
+struct Pack<float> {
+  static constexpr int kN = 4;
+  static __device__ __forceinline__ uint4 make(const float* v) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  }
+  static __device__ __forceinline__ void add(float* v, uint4 r) {
+    v[0] += __uint_as_float(r.x);
+    v[1] += __uint_as_float(r.y);
+    v[2] += __uint_as_float(r.z);
+    v[3] += __uint_as_float(r.w);
+  }
+};
+template <typename T>
+struct Pack {
+  static constexpr int kN = 8;
+  static __device__ __forceinline__ uint4 make(const float* v) {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+    return *reinterpret_cast<const uint4*>(e);
+  }
+  static __device__ __forceinline__ void add(float* v, uint4 r) {
+    const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += to_f32(e[i]);
+  }
+};
+
 // ---------------------------------------------------------------- pairs of SMs
 
 // A cluster of two CTAs owns a 256 x 256 tile.  Each CTA loads its own 128
@@ -177,11 +243,11 @@ __device__ __forceinline__ void drain_loads(uint64_t* full, uint32_t stages, uin
 namespace pair {
 
 constexpr int kBN = 256;
-constexpr int kStages = 6;
+constexpr int kStages = 5;
 constexpr int kStageBytes = kABytes + 128 * kFp8Block;
-constexpr int kOutBytes = 32 * 128;  // one warp's 32 rows x 32 f32 on the way out
+constexpr int kBoxBytes = 32 * 128;  // 32 rows x 128 bytes of results (or of the residual)
 constexpr int kOffOut = kStages * kStageBytes;
-constexpr int kOffAmax = kOffOut + 8 * kOutBytes;
+constexpr int kOffAmax = kOffOut + 8 * 2 * kBoxBytes;  // two boxes per epilogue warp
 constexpr int kOffBar = kOffAmax + 2 * kRows * 4;
 constexpr int kSmem = 1024 + kOffBar + 256;
 static_assert(kSmem <= 232448, "dynamic shared memory per block");
@@ -189,15 +255,17 @@ static_assert(kSmem <= 232448, "dynamic shared memory per block");
 template <bool GATED, typename OutT>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
-                    const __grid_constant__ CUtensorMap tmU, const __grid_constant__ Fp8GemmParams p) {
+                    const __grid_constant__ CUtensorMap tmU, const __grid_constant__ CUtensorMap tmOut,
+                    const __grid_constant__ CUtensorMap tmRes, const __grid_constant__ Fp8GemmParams p, bool boxes) {
   constexpr bool kCodes = sizeof(OutT) == 1;  // 8-bit rows out (gated)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBar);  // [kStages] even CTA: operands of both landed
   uint64_t* done = full + kStages;       // [kStages] each CTA: MMA done (stage free, partial ready)
   uint64_t* acc_empty = done + kStages;  // [2] even CTA: partial read by 16 epilogue warps
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t* res_full = acc_empty + 2;    // [8][2] each epilogue warp's boxes of the residual
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + 16);
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   uint32_t* status = p.status ? p.status : &g_fp8_status;
   const uint32_t rank = cluster_rank();
 
@@ -213,6 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&done[i], 1);
     }
     for (int i = 0; i < 2; ++i) mbar_init(&acc_empty[i], 16);
+    for (int i = 0; i < 16; ++i) mbar_init(&res_full[i], 1);
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmW);
@@ -252,27 +321,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the odd CTA's loads complete on the even CTA's barriers; the cluster
       // barrier at the end holds it until the even CTA has waited
       if (!ok && rank == 0) drain_loads(full, kStages, i, status);
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
       constexpr uint32_t idesc = idesc_e4m3_f32(2 * kRows, kBN);
-      uint32_t i = 0;
-      bool ok = true;
-      for (int64_t tile = tile0; tile < tiles && ok; tile += tile_step) {
-        for (int kb = 0; kb < kblocks; ++kb, ++i) {
-          const uint32_t s = i % kStages, buf = i & 1;
-          ok = mbar_wait(&full[s], (i / kStages) & 1, status) &&
-               mbar_wait(&acc_empty[buf], ((i >> 1) & 1) ^ 1, status);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * kStageBytes);
-          mma_block<true>(tmem_base + buf * kBN, sa, sa + kABytes, idesc);
-          tc_commit_pair(&done[s]);
-        }
-      }
+      const int64_t mine = tiles > tile0 ? (tiles - tile0 + tile_step - 1) / tile_step : 0;
+      mma_loop<true, kStages, kStageBytes, kBN>(tmem_base, idesc, smem_u32(smem), full, done, acc_empty,
+                                                static_cast<uint32_t>(mine * kblocks),
+                                                status, [](uint64_t* b) { tc_commit_pair(b); });
     }
   } else {
     regs_for_epilogue();
     const int q = warp & 3, h = (warp >> 2) - 1;  // TMEM lane quarter, column half
-    uint8_t* stage = smem + kOffOut + (warp - 4) * kOutBytes;
+    uint8_t* box = smem + kOffOut + (warp - 4) * 2 * kBoxBytes;
     float* amax = reinterpret_cast<float*>(smem + kOffAmax);  // [half][row of the tile]
     const uint32_t tlane = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * 128;
     const uint32_t empty0 = map_to_rank(&acc_empty[0], 0);
@@ -291,12 +350,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         fetch_scales<GATED>(sc, j, j, kblocks);
       }
     };
+    // Boxes of results: kBoxCols columns x this warp's 32 rows.
+    constexpr int kSize = kCodes ? 4 : static_cast<int>(sizeof(OutT));
+    constexpr int kBoxCols = 128 / kSize, kBoxes = kFeat / 2 / kBoxCols;
+    const bool res_boxes = !kCodes && !GATED && boxes && p.residual != nullptr;
+    uint64_t* res_bar = res_full + (warp - 4) * 2;
+    uint32_t res_phase = 0;  // bit b: parity of the next load into box b
+    auto fetch_residual = [&](int b, int x, int y) {  // one lane; the box is not in use
+      if (x < p.n && y < p.m) {
+        mbar_arrive_expect_tx(&res_bar[b], kBoxBytes);
+        tma_load_2d(box + b * kBoxBytes, &tmRes, &res_bar[b], x, y);
+      }
+    };
     uint32_t i = 0;
     bool ok = true;
     open_tile(tile0);
     for (int64_t tile = tile0; tile < tiles && ok; tile += tile_step) {
       const int m0 = static_cast<int>(tile / n_tiles) * 2 * kRows + static_cast<int>(rank) * kRows;
       const int f0 = static_cast<int>(tile % n_tiles) * kFeat;
+      const int row0 = m0 + q * 32, col0 = f0 + h * (kFeat / 2);  // this warp's first row and output column
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
@@ -320,16 +392,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++i;
           }
         }
+        // the first boxes of the residual, once the tile before has left them
+        if (kb0 == 0 && res_boxes && lane == 0) {
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          fetch_residual(0, col0, row0);
+          fetch_residual(1, col0 + kBoxCols, row0);
+        }
       }
       if (!ok) break;
       open_tile(tile + tile_step);  // arrives while this tile is written
 
-      const int row = m0 + q * 32 + lane;
+      const int row = row0 + lane;
       if constexpr (GATED) {
 #pragma unroll
         for (int j = 0; j < 64; ++j) acc[j] = gate(acc[j], acc[64 + j], p.act);
       }
-      const int col0 = f0 + h * (kFeat / 2);  // the thread's first output column
       if constexpr (kCodes) {
         // The 64 results of this thread and those of the thread with the same
         // row in the other half are one block of 128.
@@ -360,41 +437,81 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       } else {
-        // 32 columns at a time through shared memory, so that eight lanes
-        // write 32 consecutive elements of a row.
-        OutT* out = static_cast<OutT*>(p.out);
-        const OutT* res = static_cast<const OutT*>(p.residual);
-        const int cc = lane & 7, r0 = m0 + q * 32 + (lane >> 3);
+        if (boxes) {
+          // One box at a time: converted into shared memory (128-byte swizzle)
+          // and written by one TMA store, which clips what lies outside.
 #pragma unroll
-        for (int c = 0; c < (GATED ? 2 : 4); ++c) {
-          const int col = col0 + 32 * c + 4 * cc;
-          float4 rv[8];
+          for (int c = 0; c < kBoxes; ++c) {
+            uint8_t* b = box + (c & 1) * kBoxBytes;
+            const int x = col0 + c * kBoxCols;
+            const bool inside = x < p.n && row0 < p.m;
+            if (res_boxes) {
+              if (inside) {
+                if (!mbar_wait(&res_bar[c & 1], (res_phase >> (c & 1)) & 1, status)) ok = false;
+                res_phase ^= 1u << (c & 1);
+              }
+            } else {
+              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+              __syncwarp();
+            }
+            constexpr int kN = Pack<OutT>::kN;
 #pragma unroll
-          for (int t = 0; t < 8; ++t) {
-            const int64_t rr = r0 + 4 * t;
-            rv[t] = res ? load4(res + rr * p.ldr + col, rr < p.m ? p.n - col : 0, p.vec_r)
-                        : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < 8; ++k) {
+              uint4* at = reinterpret_cast<uint4*>(b + lane * 128 + ((k ^ (lane & 7)) << 4));
+              float* v = acc + c * kBoxCols + k * kN;
+              if (res_boxes && inside) Pack<OutT>::add(v, *at);
+              *at = Pack<OutT>::make(v);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (inside)
+                asm volatile(
+                    "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                        reinterpret_cast<uint64_t>(&tmOut)),
+                    "r"(smem_u32(b)), "r"(x), "r"(row0)
+                    : "memory");
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+              if (kBoxes > 2 && res_boxes && c + 2 < kBoxes) {
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                fetch_residual(c & 1, x + 2 * kBoxCols, row0);
+              }
+            }
           }
-          __syncwarp();
+        } else {
+          // Rows off the 16-byte boundary: 32 columns at a time through shared
+          // memory, then element by element, a lane per column.
+          OutT* out = static_cast<OutT*>(p.out);
+          const OutT* res = static_cast<const OutT*>(p.residual);
+          float* f = reinterpret_cast<float*>(box);
+          const int left = min(32, p.m - row0);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<float4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                make_float4(acc[32 * c + 4 * j], acc[32 * c + 4 * j + 1], acc[32 * c + 4 * j + 2], acc[32 * c + 4 * j + 3]);
-          __syncwarp();
+          for (int c = 0; c < kFeat / 64; ++c) {
+            __syncwarp();
 #pragma unroll
-          for (int t = 0; t < 8; ++t) {
-            const int lr = (lane >> 3) + 4 * t;
-            const int64_t rr = r0 + 4 * t;
-            float4 v = *reinterpret_cast<const float4*>(stage + lr * 128 + ((cc ^ (lr & 7)) << 4));
-            v.x += rv[t].x;
-            v.y += rv[t].y;
-            v.z += rv[t].z;
-            v.w += rv[t].w;
-            store4(out + rr * p.ldo + col, rr < p.m ? p.n - col : 0, p.vec_o, v);
+            for (int k = 0; k < 8; ++k)
+              *reinterpret_cast<uint4*>(box + lane * 128 + ((k ^ (lane & 7)) << 4)) =
+                  Pack<float>::make(acc + 32 * c + 4 * k);
+            __syncwarp();
+            const int col = col0 + 32 * c + lane;
+            if (col < p.n) {
+#pragma unroll 4
+              for (int r = 0; r < left; ++r) {
+                const int64_t rr = row0 + r;
+                float v = f[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
+                if (res) v += to_f32(res[rr * p.ldr + col]);
+                out[rr * p.ldo + col] = from_f32<OutT>(v);
+              }
+            }
           }
         }
       }
     }
+    // Stores have to finish before the CTA ends; so do residual loads that a
+    // wait that ran out left behind.
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (!ok && res_boxes)
+      for (int b = 0; b < 2; ++b) mbar_wait_limit(&res_bar[b], (res_phase >> b) & 1, status, kWaitLimitNs / 1000);
   }
 
   __syncwarp();
@@ -422,7 +539,7 @@ template <int BN>
 struct Plan {
   static constexpr int kStages = BN == 256 ? 4 : 6;
   static constexpr int kStageBytes = kABytes + BN * kFp8Block;
-  static constexpr int kBufs = static_cast<int>(kTmemCols) / BN;
+  static constexpr int kBufs = 2;
   static constexpr int kOffBar = kStages * kStageBytes;
   static constexpr int kSmem = 1024 + kOffBar + 256;
   static_assert(kSmem <= 232448, "dynamic shared memory per block");
@@ -459,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* done = full + PL::kStages;  // MMA done: stage free, partial ready
   uint64_t* acc_empty = done + PL::kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + PL::kBufs);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   uint32_t* status = p.status ? p.status : &g_fp8_status;
 
   constexpr int kFeat = GATED ? BN / 2 : BN;
@@ -510,19 +627,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                       GATED ? f0 + (c >> 1) * 64 : f0 + c * 64);
       }
       if (!ok) drain_loads(full, PL::kStages, i, status);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       constexpr uint32_t idesc = idesc_e4m3_f32(kRows, BN);
-      uint32_t i = 0;
-      for (int kb = rank; kb < kblocks; kb += split, ++i) {
-        const uint32_t s = i % PL::kStages, buf = i % PL::kBufs;
-        if (!mbar_wait(&full[s], (i / PL::kStages) & 1, status) ||
-            !mbar_wait(&acc_empty[buf], ((i / PL::kBufs) & 1) ^ 1, status))
-          break;
-        tc_fence_after();
-        const uint32_t sa = smem_u32(smem + s * PL::kStageBytes);
-        mma_block<false>(tmem_base + buf * BN, sa, sa + kABytes, idesc);
-        tc_commit(&done[s]);
-      }
+      mma_loop<false, PL::kStages, PL::kStageBytes, BN>(
+          tmem_base, idesc, smem_u32(smem), full, done, acc_empty,
+          rank < kblocks ? (kblocks - rank + split - 1) / split : 0, status, [](uint64_t* b) { tc_commit(b); });
     }
   } else {
     regs_for_epilogue();
@@ -686,6 +795,21 @@ bool codes_map(CUtensorMap* m, const uint8_t* ptr, int64_t rows, int64_t k, int6
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Results or residual [rows][ld]: boxes of 32 rows x 128 bytes, 128-byte swizzle.
+template <typename T>
+bool values_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t ld) {
+  const EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * sizeof(T)};
+  cuuint32_t box[2] = {128 / sizeof(T), 32};
+  cuuint32_t es[2] = {1, 1};
+  return enc(m, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
+             const_cast<void*>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Largest dynamic shared memory, once per device and kernel.
 template <auto KERNEL>
 cudaError_t allow_smem(int bytes) {
@@ -723,8 +847,18 @@ cudaError_t launch_pair(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
   constexpr int kFeat = GATED ? pair::kBN / 2 : pair::kBN;
   const int64_t tiles = static_cast<int64_t>((p.m + 2 * kRows - 1) / (2 * kRows)) * ((p.n + kFeat - 1) / kFeat);
   const int clusters = static_cast<int>(std::min<int64_t>(tiles, std::max(1, num_sms / 2)));
+  // results by TMA boxes where rows (and the residual's) start at multiples of 16 bytes
+  CUtensorMap to = ta, tr = ta;
+  bool boxes = false;
+  if constexpr (sizeof(OutT) > 1) {
+    boxes = p.box_o && (!p.residual || p.box_r);
+    if (boxes && (!values_map<OutT>(&to, p.out, p.m, p.n, p.ldo) ||
+                  (p.residual && !values_map<OutT>(&tr, p.residual, p.m, p.n, p.ldr))))
+      return cudaErrorInvalidValue;
+  }
   const cudaLaunchAttribute attr = cluster_of(2);
-  return launch_pdl(kernel, dim3(2 * clusters), dim3(kThreads), pair::kSmem, st, &attr, 1, ta, tw, tu, p);
+  return launch_pdl(kernel, dim3(2 * clusters), dim3(kThreads), pair::kSmem, st, &attr, 1, ta, tw, tu, to, tr, p,
+                    boxes);
 }
 
 template <bool GATED, typename OutT, int BN>

@@ -16,6 +16,7 @@ struct Fp8GemmParams {
   int m, n, k;
   int act;                           // WC_ACT_*, gated only
   bool vec_o, vec_r;                 // output / residual rows aligned to four elements
+  bool box_o, box_r;                 // ... and to 16 bytes
   uint32_t* status;                  // wait timeouts; null: the library's own word
 };
 
