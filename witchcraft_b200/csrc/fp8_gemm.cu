@@ -132,40 +132,13 @@ __device__ __forceinline__ void tmem_ld32_wait(uint32_t (&r)[32]) {
                : "memory");
 }
 
-// acc[] += s0 * (first half) or s1 * (second half) of the 32 CHUNKS columns at
-// taddr; calls `read` once all of them are in registers.  Scalar
-// multiply-adds: the packed form needs register pairs that the TMEM load's
-// results have to be moved into, which cost more than it saved (8192 x 4096 x
-// 8192: 374 us packed, 353 us scalar).
-template <int CHUNKS, typename Read>
-__device__ __forceinline__ void add_block(uint32_t taddr, float s0, float s1, float (&acc)[32 * CHUNKS], Read read) {
-  uint32_t r[2][32];
-  auto fma = [&](int c) {
-    const float s = 2 * c < CHUNKS ? s0 : s1;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) acc[32 * c + j] = __fmaf_rn(__uint_as_float(r[c & 1][j]), s, acc[32 * c + j]);
-  };
-  tmem_ld32_issue(taddr, r[0]);
-  tmem_ld32_issue(taddr + 32, r[1]);
-#pragma unroll
-  for (int c = 0; c < CHUNKS; c += 2) {
-    tmem_ld32_wait(r[0]);
-    tmem_ld32_wait(r[1]);
-    if (c + 2 >= CHUNKS) read();
-    fma(c);
-    if (c + 2 < CHUNKS) tmem_ld32_issue(taddr + 32 * (c + 2), r[0]);
-    fma(c + 1);
-    if (c + 2 < CHUNKS) tmem_ld32_issue(taddr + 32 * (c + 3), r[1]);
-  }
-}
-
-// The scales of one thread's row and columns, block by block, two blocks
-// ahead of their use: a load from L2 takes about as long as a block.  The
-// loads are volatile, or the compiler moves them down to their use.
+// The scales of one thread's row and columns, fetched one block ahead of
+// their use.  The loads are volatile, or the compiler moves them down to it.
+// Rows and columns outside the matrix use the last ones' scales (their results
+// are not stored).
 struct Scales {
-  const float *a, *w, *u;  // the row's, the columns', the up columns'
-  bool live;
-  float va[2], vw[2], vu[2];
+  const float *a, *w, *u;  // the row's, the columns', the up columns' next scale
+  float va, vw, vu;
 };
 __device__ __forceinline__ float load_ahead(const float* p) {
   float v;
@@ -173,12 +146,85 @@ __device__ __forceinline__ float load_ahead(const float* p) {
   return v;
 }
 template <bool GATED>
-__device__ __forceinline__ void fetch_scales(Scales& s, int slot, int kb, int kblocks) {
-  if (s.live && kb < kblocks) {
-    s.va[slot] = load_ahead(s.a + kb);
-    s.vw[slot] = load_ahead(s.w + kb);
-    if (GATED) s.vu[slot] = load_ahead(s.u + kb);
+__device__ __forceinline__ void fetch_scales(Scales& s, int step) {
+  s.va = load_ahead(s.a);
+  s.vw = load_ahead(s.w);
+  s.a += step;
+  s.w += step;
+  if (GATED) {
+    s.vu = load_ahead(s.u);
+    s.u += step;
   }
+}
+template <bool GATED>
+__device__ __forceinline__ Scales scales_at(const Fp8GemmParams& p, int row, int nb, int kb) {
+  row = min(row, p.m - 1);
+  nb = min(nb, (p.n - 1) / kFp8Block);
+  Scales s{};
+  s.a = p.sa + row * p.ldsa + kb;
+  s.w = p.sw + nb * p.ldsw + kb;
+  if (GATED) s.u = p.sup + nb * p.ldsup + kb;
+  return s;
+}
+
+// Position in the ring of operand stages, whose `done` barriers also say that
+// a block's partial is complete.
+template <int STAGES>
+struct Ring {
+  uint32_t i = 0, stage = 0, parity = 0;  // blocks so far, and where the next one is
+  __device__ __forceinline__ void next() {
+    ++i;
+    if (++stage == STAGES) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+// acc[] = sum over `blocks` (>= 1) blocks, `step` apart, of scale * partial for
+// this thread's row and 32 CHUNKS columns (taddr of partial 0; partial 1 lies
+// BN columns on).  sc holds the first block's scales.  The columns come 32 at
+// a time, the next 32 loading while these are added.  The multiply-adds are
+// scalar: the packed form needs register pairs that a TMEM load's results have
+// to be moved into.  What matters most here is that nothing spills: keeping
+// the next block's first columns in flight across the loop's end made the
+// whole product twice as slow.  `read(buf)` once a partial is in registers.
+// False if a wait ran out.
+template <bool GATED, int CHUNKS, int STAGES, int BN, typename Read>
+__device__ __forceinline__ bool sum_blocks(float (&acc)[32 * CHUNKS], Scales& sc, int blocks, int step, uint32_t taddr,
+                                           uint64_t* done, Ring<STAGES>& ring, uint32_t* status, Read read) {
+  static_assert(CHUNKS == 2 || CHUNKS == 4, "two register sets");
+  uint32_t r[2][32];
+#pragma unroll
+  for (int j = 0; j < 32 * CHUNKS; ++j) acc[j] = 0.f;
+#pragma unroll 1
+  for (int left = blocks; left > 0; --left) {
+    const float s0 = sc.va * sc.vw, s1 = GATED ? sc.va * sc.vu : s0;
+    if (left > 1) fetch_scales<GATED>(sc, step);
+    if (!__all_sync(0xFFFFFFFFu, mbar_wait(&done[ring.stage], ring.parity, status))) return false;
+    tc_fence_after();
+    const uint32_t at = taddr + (ring.i & 1) * BN;
+    auto add = [&](int c) {
+      const float s = 2 * c < CHUNKS ? s0 : s1;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) acc[32 * c + e] = __fmaf_rn(__uint_as_float(r[c & 1][e]), s, acc[32 * c + e]);
+    };
+    tmem_ld32_issue(at, r[0]);
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      tmem_ld32_wait(r[c & 1]);
+      if (c + 1 < CHUNKS) {
+        tmem_ld32_issue(at + 32 * (c + 1), r[(c + 1) & 1]);
+      } else {
+        tc_fence_before();
+    __syncwarp();
+    read(ring.i & 1);
+      }
+      add(c);
+    }
+    ring.next();
+  }
+  return true;
 }
 
 // act(g) u, both activations in the form g / (1 + exp(-z)): z = g (SiLU), or
@@ -267,13 +313,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + 16);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   uint32_t* status = p.status ? p.status : &g_fp8_status;
-  const uint32_t rank = cluster_rank();
+  // a cluster is two neighbours of the grid; said with blockIdx, the compiler
+  // knows that what follows from it is the same for the whole warp
+  const int rank = blockIdx.x & 1;
 
   constexpr int kFeat = GATED ? kBN / 2 : kBN;  // output columns per tile
   const int kblocks = (p.k + kFp8Block - 1) / kFp8Block;
   const int m_tiles = (p.m + 2 * kRows - 1) / (2 * kRows), n_tiles = (p.n + kFeat - 1) / kFeat;
-  const int64_t tiles = static_cast<int64_t>(m_tiles) * n_tiles;
-  const int64_t tile0 = cluster_id(), tile_step = num_clusters();
+  const int tiles = m_tiles * n_tiles;
+  const int tile0 = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -303,9 +351,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0 && lane == 0) {
       uint32_t i = 0;
       bool ok = true;
-      for (int64_t tile = tile0; tile < tiles && ok; tile += tile_step) {
-        const int m0 = static_cast<int>(tile / n_tiles) * 2 * kRows + static_cast<int>(rank) * kRows;
-        const int f0 = static_cast<int>(tile % n_tiles) * kFeat + static_cast<int>(rank) * (kFeat / 2);
+      for (int tile = tile0; tile < tiles && ok; tile += tile_step) {
+        const int m0 = (tile / n_tiles) * 2 * kRows + rank * kRows;
+        const int f0 = (tile % n_tiles) * kFeat + rank * (kFeat / 2);
         for (int kb = 0; kb < kblocks; ++kb, ++i) {
           const uint32_t s = i % kStages;
           if (!(ok = mbar_wait(&done[s], ((i / kStages) & 1) ^ 1, status))) break;
@@ -323,9 +371,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok && rank == 0) drain_loads(full, kStages, i, status);
     } else if (warp == 1 && rank == 0) {
       constexpr uint32_t idesc = idesc_e4m3_f32(2 * kRows, kBN);
-      const int64_t mine = tiles > tile0 ? (tiles - tile0 + tile_step - 1) / tile_step : 0;
+      const int mine = tiles > tile0 ? (tiles - tile0 + tile_step - 1) / tile_step : 0;
       mma_loop<true, kStages, kStageBytes, kBN>(tmem_base, idesc, smem_u32(smem), full, done, acc_empty,
-                                                static_cast<uint32_t>(mine * kblocks),
+                                                static_cast<uint32_t>(mine) * kblocks,
                                                 status, [](uint64_t* b) { tc_commit_pair(b); });
     }
   } else {
@@ -335,20 +383,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* amax = reinterpret_cast<float*>(smem + kOffAmax);  // [half][row of the tile]
     const uint32_t tlane = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * 128;
     const uint32_t empty0 = map_to_rank(&acc_empty[0], 0);
-    Scales sc{};
-    auto open_tile = [&](int64_t tile) {  // its scales' addresses and first two blocks
-      const int row = static_cast<int>(tile / n_tiles) * 2 * kRows + static_cast<int>(rank) * kRows + q * 32 + lane;
-      const int f0 = static_cast<int>(tile % n_tiles) * kFeat;
-      const int nb = GATED ? f0 / kFp8Block : f0 / kFp8Block + h;  // block of weight rows
-      sc.live = tile < tiles && row < p.m && nb * kFp8Block < p.n;
-      sc.a = p.sa + row * p.ldsa;
-      sc.w = p.sw + nb * p.ldsw;
-      if (GATED) sc.u = p.sup + nb * p.ldsup;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        sc.va[j] = sc.vw[j] = sc.vu[j] = 0.f;
-        fetch_scales<GATED>(sc, j, j, kblocks);
-      }
+    // A tile's scales, the first block's on their way (past the last tile: the last one's).
+    auto open_tile = [&](int tile) {
+      tile = min(tile, tiles - 1);
+      const int f0 = (tile % n_tiles) * kFeat;
+      Scales s = scales_at<GATED>(
+          p, (tile / n_tiles) * 2 * kRows + rank * kRows + q * 32 + lane,
+          f0 / kFp8Block + (GATED ? 0 : h), 0);
+      fetch_scales<GATED>(s, 1);
+      return s;
     };
     // Boxes of results: kBoxCols columns x this warp's 32 rows.
     constexpr int kSize = kCodes ? 4 : static_cast<int>(sizeof(OutT));
@@ -362,45 +405,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_2d(box + b * kBoxBytes, &tmRes, &res_bar[b], x, y);
       }
     };
-    uint32_t i = 0;
+    Ring<kStages> ring;
     bool ok = true;
-    open_tile(tile0);
-    for (int64_t tile = tile0; tile < tiles && ok; tile += tile_step) {
-      const int m0 = static_cast<int>(tile / n_tiles) * 2 * kRows + static_cast<int>(rank) * kRows;
-      const int f0 = static_cast<int>(tile % n_tiles) * kFeat;
+    Scales sc = open_tile(tile0);
+    for (int tile = tile0; tile < tiles && ok; tile += tile_step) {
+      const int m0 = (tile / n_tiles) * 2 * kRows + rank * kRows;
+      const int f0 = (tile % n_tiles) * kFeat;
       const int row0 = m0 + q * 32, col0 = f0 + h * (kFeat / 2);  // this warp's first row and output column
-      float acc[128];
-#pragma unroll
-      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
-      for (int kb0 = 0; kb0 < kblocks && ok; kb0 += 2) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int kb = kb0 + j;
-          if (kb < kblocks && ok) {
-            const uint32_t buf = i & 1, st = i % kStages;
-            const float s0 = sc.va[j] * sc.vw[j], s1 = GATED ? sc.va[j] * sc.vu[j] : s0;
-            fetch_scales<GATED>(sc, j, kb + 2, kblocks);
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&done[st], (i / kStages) & 1, status));
-            if (ok) {
-              tc_fence_after();
-              add_block<4>(tlane + buf * kBN, s0, s1, acc, [&] {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_remote(empty0 + buf * 8);
-              });
-            }
-            ++i;
-          }
-        }
-        // the first boxes of the residual, once the tile before has left them
-        if (kb0 == 0 && res_boxes && lane == 0) {
-          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          fetch_residual(0, col0, row0);
-          fetch_residual(1, col0 + kBoxCols, row0);
-        }
+      // the residual's first boxes, once the tile before has left them
+      if (res_boxes && lane == 0) {
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        fetch_residual(0, col0, row0);
+        fetch_residual(1, col0 + kBoxCols, row0);
       }
+      float acc[128];
+      ok = sum_blocks<GATED, 4, kStages, kBN>(
+          acc, sc, kblocks, 1, tlane, done, ring, status,
+          [&](uint32_t buf) {
+            if (lane == 0) mbar_arrive_remote(empty0 + buf * 8);
+          });
       if (!ok) break;
-      open_tile(tile + tile_step);  // arrives while this tile is written
+      sc = open_tile(tile + tile_step);  // arrives while this tile is written
 
       const int row = row0 + lane;
       if constexpr (GATED) {
@@ -539,7 +564,6 @@ template <int BN>
 struct Plan {
   static constexpr int kStages = BN == 256 ? 4 : 6;
   static constexpr int kStageBytes = kABytes + BN * kFp8Block;
-  static constexpr int kBufs = 2;
   static constexpr int kOffBar = kStages * kStageBytes;
   static constexpr int kSmem = 1024 + kOffBar + 256;
   static_assert(kSmem <= 232448, "dynamic shared memory per block");
@@ -575,16 +599,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + PL::kOffBar);
   uint64_t* done = full + PL::kStages;  // MMA done: stage free, partial ready
   uint64_t* acc_empty = done + PL::kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + PL::kBufs);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   uint32_t* status = p.status ? p.status : &g_fp8_status;
 
   constexpr int kFeat = GATED ? BN / 2 : BN;
   const int kblocks = (p.k + kFp8Block - 1) / kFp8Block;
   const int n_tiles = (p.n + kFeat - 1) / kFeat;
-  const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
-  const int64_t tile = blockIdx.x / split;
-  const int m0 = static_cast<int>(tile / n_tiles) * kRows, f0 = static_cast<int>(tile % n_tiles) * kFeat;
+  const int rank = blockIdx.x % split, tile = blockIdx.x / split;  // a cluster is `split` neighbours of the grid
+  const int m0 = (tile / n_tiles) * kRows, f0 = (tile % n_tiles) * kFeat;
   const int rows = min(kRows, p.m - m0);
   const int epi_warps = 2 * ((rows + 31) / 32);  // warps whose lanes hold rows of the matrix
 
@@ -593,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&full[i], 1);
       mbar_init(&done[i], 1);
     }
-    for (int i = 0; i < PL::kBufs; ++i) mbar_init(&acc_empty[i], epi_warps);
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_empty[i], epi_warps);
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmW);
@@ -631,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t idesc = idesc_e4m3_f32(kRows, BN);
       mma_loop<false, PL::kStages, PL::kStageBytes, BN>(
           tmem_base, idesc, smem_u32(smem), full, done, acc_empty,
-          rank < kblocks ? (kblocks - rank + split - 1) / split : 0, status, [](uint64_t* b) { tc_commit(b); });
+          (kblocks - rank + split - 1) / split, status, [](uint64_t* b) { tc_commit(b); });
     }
   } else {
     regs_for_epilogue();
@@ -640,39 +663,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t tlane = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * (BN / 2);
       const int lrow = q * 32 + lane, row = m0 + lrow;
       const int nb = f0 / kFp8Block + (GATED || BN == 128 ? 0 : h);  // block of weight rows
-      Scales sc{};
-      sc.live = lrow < rows && nb * kFp8Block < p.n;
-      sc.a = p.sa + row * p.ldsa;
-      sc.w = p.sw + nb * p.ldsw;
-      if (GATED) sc.u = p.sup + nb * p.ldsup;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) fetch_scales<GATED>(sc, j, rank + j * split, kblocks);
+      const int blocks = (kblocks - rank + split - 1) / split;  // at least one: split <= kblocks
+      Scales sc = scales_at<GATED>(p, row, nb, rank);
       float acc[32 * kChunks];
-#pragma unroll
-      for (int j = 0; j < 32 * kChunks; ++j) acc[j] = 0.f;
-      uint32_t i = 0;
-      bool ok = true;
-      for (int kb0 = rank; kb0 < kblocks && ok; kb0 += 2 * split) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int kb = kb0 + j * split;
-          if (kb < kblocks && ok) {
-            const uint32_t buf = i % PL::kBufs, st = i % PL::kStages;
-            const float s0 = sc.va[j] * sc.vw[j], s1 = GATED ? sc.va[j] * sc.vu[j] : s0;
-            fetch_scales<GATED>(sc, j, kb + 2 * split, kblocks);
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&done[st], (i / PL::kStages) & 1, status));
-            if (ok) {
-              tc_fence_after();
-              add_block<kChunks>(tlane + buf * BN, s0, s1, acc, [&] {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_empty[buf]);
-              });
-            }
-            ++i;
-          }
-        }
-      }
+      Ring<PL::kStages> ring;
+      fetch_scales<GATED>(sc, split);
+      sum_blocks<GATED, kChunks, PL::kStages, BN>(
+          acc, sc, blocks, split, tlane, done, ring, status,
+          [&](uint32_t buf) {
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+          });
       // The last partial was committed after every MMA of this CTA, so the
       // operand stages are free for the sums.
 #pragma unroll
@@ -835,6 +835,8 @@ cudaLaunchAttribute cluster_of(int n) {
   return a;
 }
 
+int clusters_of(int num_sms) { return std::max(1, num_sms / 2); }
+
 template <bool GATED, typename OutT>
 cudaError_t launch_pair(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
   constexpr auto kernel = pair::fp8_pair_kernel<GATED, OutT>;
@@ -846,7 +848,9 @@ cudaError_t launch_pair(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
     return cudaErrorInvalidValue;
   constexpr int kFeat = GATED ? pair::kBN / 2 : pair::kBN;
   const int64_t tiles = static_cast<int64_t>((p.m + 2 * kRows - 1) / (2 * kRows)) * ((p.n + kFeat - 1) / kFeat);
-  const int clusters = static_cast<int>(std::min<int64_t>(tiles, std::max(1, num_sms / 2)));
+  if (tiles > 0x40000000 || tiles * ((p.k + kFp8Block - 1) / kFp8Block) > 0xFFFFFFFFll * clusters_of(num_sms))
+    return cudaErrorInvalidValue;  // tile and block numbers are 32-bit
+  const int clusters = static_cast<int>(std::min<int64_t>(tiles, clusters_of(num_sms)));
   // results by TMA boxes where rows (and the residual's) start at multiples of 16 bytes
   CUtensorMap to = ta, tr = ta;
   bool boxes = false;
@@ -892,7 +896,7 @@ cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
 #ifdef WC_FP8_SWEEP
   if (const char* f = getenv("WC_FP8_FORCE")) {
     if (atoi(f) == 0) return launch_pair<GATED, OutT>(p, num_sms, st);
-    split = atoi(f);
+    split = std::min<int>(atoi(f), kblocks);
   }
 #endif
   return launch_tile<GATED, OutT, BN>(p, split, st);
