@@ -4,7 +4,8 @@ Every CUDA translation unit is compiled for sm_100a only
 (`-gencode arch=compute_100a,code=sm_100a`); the host C++ parts with g++.
 The library links the CUDA runtime statically and reaches the driver's
 cuTensorMapEncodeTiled through cudaGetDriverEntryPointByVersion, so it needs
-no libcuda at link time and no torch at all.
+no libcuda at link time and no torch at all.  The torch binding of the 8-bit
+operators is a second, small library, `witchcraft_b200/_fp8_torch.so`.
 
 Usage: python -m witchcraft_b200.build   (or witchcraft_b200.build.build())
 """
@@ -18,6 +19,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libwc_t5cuda.so")
+TORCH_BINDING = os.path.join(HERE, "_fp8_torch.so")
 BUILD_DIR = os.path.join(HERE, "_build")
 
 CUDA_SOURCES = ["gemm_q4k.cu", "gemm2_q4k.cu", "gemv_q4k.cu", "attention_tc.cu", "attention_small.cu", "elementwise.cu",
@@ -72,7 +74,26 @@ def build(verbose: bool = False, force: bool = False) -> str:
             _run(["g++", "-O2", "-std=c++17", "-fPIC", "-I/usr/local/cuda/include", "-c", s, "-o", o])
     if force or _stale(LIB, objs):
         _run([nvcc, *ARCH, "-shared", "-Xcompiler", "-fPIC", "-cudart", "static", "-o", LIB, *objs])
+    build_torch_binding(force)
     return LIB
+
+
+def build_torch_binding(force: bool = False) -> str:
+    """The torch binding of the 8-bit operators (witchcraft_b200/fp8.py); the
+    library itself needs no torch."""
+    src = os.path.join(CSRC, "fp8_torch.cpp")
+    header = os.path.join(os.path.dirname(HERE), "include", "wc_fp8.h")
+    if force or _stale(TORCH_BINDING, [src, header]):
+        import sysconfig
+
+        import torch
+        from torch.utils.cpp_extension import include_paths, library_paths
+        inc = [f"-I{d}" for d in include_paths()] + [f"-I{sysconfig.get_paths()['include']}", "-I/usr/local/cuda/include"]
+        abi = int(torch.compiled_with_cxx11_abi())
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *inc, src, "-o",
+              TORCH_BINDING, *[f"-L{d}" for d in library_paths()], "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+              "-ltorch_python"])
+    return TORCH_BINDING
 
 
 def build_oracle() -> str:
