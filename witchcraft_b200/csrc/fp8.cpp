@@ -32,6 +32,8 @@ int type_size(int t) { return t == WC_T_F32 ? 4 : t == WC_T_E4M3 ? 1 : 2; }
 bool aligned(const void* p, int64_t ld, int bytes, int type) {  // rows start at multiples of `bytes`
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (ld * type_size(type)) % bytes == 0;
 }
+// rows of eight elements at a time: 16-byte accesses
+bool vec8(const void* p, int64_t ld, int type) { return aligned(p, ld, 16, type) && ld % 8 == 0; }
 bool vec4(const void* p, int64_t ld, int type) { return aligned(p, ld, 4 * type_size(type), type); }
 bool natural(const void* p, int type) { return reinterpret_cast<uintptr_t>(p) % type_size(type) == 0; }
 int64_t blocks(int64_t k) { return (k + 127) / 128; }
@@ -91,7 +93,7 @@ int quantize(bool weight, const void* x, int type, int64_t m, int64_t k, int64_t
   p.ldx = ldx;
   p.ldc = ldc;
   p.lds = lds;
-  p.vec_x = vec4(x, ldx, type);
+  p.vec_x = vec8(x, ldx, type);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return done(weight ? fp8_weight_launch(type, p, st) : fp8_rows_launch(type, p, st), "quantisation launch");
 }
@@ -165,9 +167,9 @@ extern "C" int wc_fp8_rmsnorm(const void* d_x, int x_type, int64_t ldx, const vo
   p.ldc = ldc;
   p.lds = lds;
   p.eps = eps;
-  p.vec_x = vec4(d_x, ldx, x_type);
-  p.vec_d = d_delta && vec4(d_delta, ldd, delta_type);
-  p.vec_s = d_delta && vec4(d_sum, ldsum, x_type);
+  p.vec_x = vec8(d_x, ldx, x_type);
+  p.vec_d = d_delta && vec8(d_delta, ldd, delta_type);
+  p.vec_s = d_delta && vec8(d_sum, ldsum, x_type);
   p.vec_w = reinterpret_cast<uintptr_t>(d_w) % 16 == 0;
   return done(fp8_rmsnorm_launch(x_type, delta_type, p, static_cast<cudaStream_t>(stream)), "rmsnorm launch");
 }

@@ -10,15 +10,23 @@ namespace wc {
 constexpr int kFp8Block = 128;      // columns (and weight rows) that share a scale
 constexpr float kE4M3Max = 448.0f;  // largest finite e4m3 value
 
-// The scale of a block whose largest magnitude is amax (NaN stays NaN), and
-// what its values are multiplied by.  The floor keeps the reciprocal finite;
-// a block of zeros gets codes of zero.  inf: scale inf, factor 0, so finite
-// values become 0 * inf and infinite ones NaN codes.
+// The scale of a block whose largest magnitude is amax (NaN stays NaN): the
+// product with 1 / 448 corrected by its remainder, the rounded quotient but
+// for rare last bits.  The floor keeps the reciprocal finite; a block of zeros
+// gets codes of zero.
 __device__ __forceinline__ float fp8_scale(float amax) {
-  const float s = amax * (1.0f / kE4M3Max);
+  constexpr float c = 1.0f / kE4M3Max;
+  float s = amax * c;
+  if (amax < 3.0e38f) s = __fmaf_rn(__fmaf_rn(-kE4M3Max, s, amax), c, s);  // (not inf - inf)
   return s < 1.17549435e-38f ? 1.17549435e-38f : s;
 }
-__device__ __forceinline__ float fp8_factor(float scale) { return __fdividef(1.0f, scale); }
+// What the block's values are multiplied by: 1 / scale, the approximate
+// reciprocal after one Newton step.  scale = inf: 0, so that finite values
+// become 0 * inf and infinite ones NaN codes.
+__device__ __forceinline__ float fp8_factor(float scale) {
+  const float f = __fdividef(1.0f, scale);
+  return f == 0.0f ? 0.0f : __fmaf_rn(__fmaf_rn(-scale, f, 1.0f), f, f);
+}
 
 // Maximum that keeps a NaN (fmaxf drops it).
 __device__ __forceinline__ float max_nan(float a, float b) {

@@ -1,12 +1,12 @@
 // Rows and weights to 8 bits, and the RMSNorm with the residual add that
-// writes 8-bit rows.  All are bound by the bytes they read and write.
+// writes 8-bit rows.  All are bound by the bytes they read and write, if only
+// just: scaling, the maximum and the conversion are about ten instructions an
+// element, so what a block costs beside them is shared by eight elements.
 //
-// One warp handles one block of 128 columns at a time, four consecutive
-// elements per lane, so the block's maximum is one warp reduction and every
-// access of the warp is one contiguous run (512 B of f32, 256 B of 16-bit
-// values, 128 B of codes).  VEC: every row is aligned to four elements and k
-// is a multiple of four, so an access is either whole or absent; the other
-// form takes the edge element by element.
+// Sixteen lanes handle one block of 128 columns, eight consecutive elements
+// each (16 bytes of 16-bit values), and a warp two blocks at a time.  VEC: every
+// row is aligned to eight elements and k is a multiple of eight, so an access
+// is either whole or absent; the other form takes the edge element by element.
 #include "fp8.cuh"
 #include "fp8_rows.h"
 
@@ -15,13 +15,23 @@ namespace wc {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kRowsHeld = 4;  // blocks of a row that one warp of fp8_rows_kernel loads at once
+constexpr int kUnit = 2 * kFp8Block;  // columns a warp takes at a time
+constexpr int kHeld = 4;              // units of a row that a warp loads at once
 
-__device__ __forceinline__ float max4_nan(float4 v) {
-  return max_nan(max_nan(fabsf(v.x), fabsf(v.y)), max_nan(fabsf(v.z), fabsf(v.w)));
+struct Eight {
+  float v[8];
+};
+
+__device__ __forceinline__ float max_abs(const Eight& x) {
+  float m = fabsf(x.v[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(x.v[i]));
+  return m;
 }
-__device__ __forceinline__ uint32_t codes4(float4 v, float f) {
-  return pack_e4m3x4(v.x * f, v.y * f, v.z * f, v.w * f);
+__device__ __forceinline__ float half_warp_max_nan(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
 }
 __device__ __forceinline__ float warp_total(float v) {
 #pragma unroll
@@ -29,62 +39,107 @@ __device__ __forceinline__ float warp_total(float v) {
   return v;
 }
 
-// Four elements as they are stored, so that a row waiting in registers takes
-// no more of them than its type needs.
+// Eight elements as they are stored.
 template <typename T>
-struct Raw4 {
-  T e[4];
+struct Raw8 {
+  uint4 u;
 };
 template <>
-struct Raw4<float> {
-  float4 e;
+struct Raw8<float> {
+  float4 a, b;
 };
-template <typename T>
-__device__ __forceinline__ float4 widen(const Raw4<T>& r) {
-  if constexpr (sizeof(T) == 4)
-    return r.e;
-  else
-    return make_float4(to_f32(r.e[0]), to_f32(r.e[1]), to_f32(r.e[2]), to_f32(r.e[3]));
+__device__ __forceinline__ Eight widen(const Raw8<float>& r) {
+  return Eight{{r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w}};
 }
-template <bool VEC, typename T>
-__device__ __forceinline__ Raw4<T> get4(const T* p, int left) {
-  Raw4<T> r;
-  if constexpr (VEC) {
-    if constexpr (sizeof(T) == 4) {
-      r.e = left > 0 ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
-    } else {
-      const uint2 u = left > 0 ? *reinterpret_cast<const uint2*>(p) : make_uint2(0u, 0u);
-      *reinterpret_cast<uint2*>(&r) = u;
-    }
-  } else {
-    if constexpr (sizeof(T) == 4) {
-      r.e = load4(p, left, false);
-    } else {
+__device__ __forceinline__ Eight widen(const Raw8<__half>& r) {
+  const uint32_t w[4] = {r.u.x, r.u.y, r.u.z, r.u.w};
+  Eight e;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r.e[i] = left > i ? p[i] : from_f32<T>(0.f);
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    e.v[2 * i] = f.x;
+    e.v[2 * i + 1] = f.y;
+  }
+  return e;
+}
+__device__ __forceinline__ Eight widen(const Raw8<__nv_bfloat16>& r) {
+  const uint32_t w[4] = {r.u.x, r.u.y, r.u.z, r.u.w};
+  Eight e;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    e.v[2 * i] = __uint_as_float(w[i] << 16);
+    e.v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+  return e;
+}
+// Eight elements at p, of which `left` belong to the row; zeros past it.
+template <bool VEC, typename T>
+__device__ __forceinline__ Raw8<T> get8(const T* p, int left) {
+  Raw8<T> r;
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (VEC) {
+      r.a = r.b = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (left > 0) {
+        r.a = reinterpret_cast<const float4*>(p)[0];
+        r.b = reinterpret_cast<const float4*>(p)[1];
+      }
+    } else {
+      r.a = load4(p, left, false);
+      r.b = load4(p + 4, static_cast<int64_t>(left) - 4, false);
     }
+  } else if constexpr (VEC) {
+    r.u = left > 0 ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
+  } else {
+    const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (left > 2 * i ? e[2 * i] : 0u) | (left > 2 * i + 1 ? e[2 * i + 1] : 0u) << 16;
+    r.u = make_uint4(w[0], w[1], w[2], w[3]);
   }
   return r;
 }
 template <bool VEC, typename T>
-__device__ __forceinline__ void put4(T* p, int left, float4 v) {
-  if (!VEC) {
-    store4(p, left, false, v);
-  } else if (left > 0) {
-    store4(p, 4, true, v);
+__device__ __forceinline__ void put8(T* p, int left, const Eight& x) {
+  if constexpr (VEC) {
+    if (left <= 0) return;
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(x.v[4], x.v[5], x.v[6], x.v[7]);
+    } else {
+      T e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x.v[i]);
+      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (left > i) p[i] = from_f32<T>(x.v[i]);
   }
 }
+// The codes of eight values times f.
 template <bool VEC>
-__device__ __forceinline__ void put_codes(uint8_t* p, int left, uint32_t c) {
-  if (!VEC) {
-    store_codes4(p, left, c);
-  } else if (left > 0) {
-    *reinterpret_cast<uint32_t*>(p) = c;
+__device__ __forceinline__ void put_codes8(uint8_t* p, int left, const Eight& x, float f) {
+  const uint32_t a = pack_e4m3x4(x.v[0] * f, x.v[1] * f, x.v[2] * f, x.v[3] * f);
+  const uint32_t b = pack_e4m3x4(x.v[4] * f, x.v[5] * f, x.v[6] * f, x.v[7] * f);
+  if (left >= 8) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
+  } else if (!VEC) {
+    store_codes4(p, left, a);
+    store_codes4(p + 4, static_cast<int64_t>(left) - 4, b);
   }
+}
+// Quantises one unit of a row: eight values of this lane, of which `left`
+// belong to the row.
+template <bool VEC>
+__device__ __forceinline__ void put_unit(uint8_t* codes, float* scale, int lane, int left, const Eight& x) {
+  const float s = fp8_scale(half_warp_max_nan(max_abs(x)));
+  if ((lane & 15) == 0 && left > 0) *scale = s;
+  put_codes8<VEC>(codes, left, x, fp8_factor(s));
 }
 
-// Blocks are independent: one warp per kRowsHeld blocks of a row, all loads
-// issued first.
+// Blocks are independent: one warp per kHeld units of a row, all loads issued
+// first.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * kWarps) fp8_rows_kernel(const __grid_constant__ Fp8RowsParams p, int groups) {
   pdl_wait();
@@ -93,70 +148,54 @@ __global__ void __launch_bounds__(32 * kWarps) fp8_rows_kernel(const __grid_cons
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   const int64_t row = groups == 1 ? unit : unit / groups;
   if (row >= p.m) return;
-  const int b0 = static_cast<int>(unit - row * groups) * kRowsHeld;
-  const int64_t c0 = static_cast<int64_t>(b0) * kFp8Block + lane * 4;
-  const int left = static_cast<int>(p.k - c0);
+  const int c0 = static_cast<int>(unit - row * groups) * (kHeld * kUnit) + lane * 8;
+  const int left = static_cast<int>(p.k) - c0;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx + c0;
   uint8_t* codes = p.codes + row * p.ldc + c0;
-  Raw4<T> v[kRowsHeld];
+  float* scales = p.scales + row * p.lds + c0 / kFp8Block;
+  Raw8<T> v[kHeld];
 #pragma unroll
-  for (int g = 0; g < kRowsHeld; ++g) v[g] = get4<VEC>(x + g * kFp8Block, left - g * kFp8Block);
-  float mine = 0.f;
+  for (int g = 0; g < kHeld; ++g) v[g] = get8<VEC>(x + g * kUnit, left - g * kUnit);
 #pragma unroll
-  for (int g = 0; g < kRowsHeld; ++g) {
-    const float4 y = widen(v[g]);
-    const float s = fp8_scale(warp_max_nan(max4_nan(y)));
-    if (lane == g) mine = s;
-    put_codes<VEC>(codes + g * kFp8Block, left - g * kFp8Block, codes4(y, fp8_factor(s)));
+  for (int g = 0; g < kHeld; ++g) {
+    if (left - g * kUnit + lane * 8 <= 0) break;  // the whole unit is past the row
+    put_unit<VEC>(codes + g * kUnit, scales + g * 2, lane, left - g * kUnit, widen(v[g]));
   }
-  // lane's own block: left + 4 lane columns remain from the group's start
-  if (lane < kRowsHeld && left + lane * 4 > lane * kFp8Block) p.scales[row * p.lds + b0 + lane] = mine;
 }
 
-// One row by WPR warps.  HELD blocks per warp stay in registers between the
-// sum of squares and the scaling (rows up to WPR * HELD * 128 columns); a
-// wider row (WIDE) is read again for the second pass.
-template <typename TX, typename TD, bool DELTA, bool VEC, int WPR, int HELD, bool WIDE>
-__global__ void __launch_bounds__(32 * kWarps, WIDE ? 2 : 4)
-    fp8_rmsnorm_kernel(const __grid_constant__ Fp8RowsParams p) {
+// One row by WPR warps, its kHeld units per warp in registers between the sum
+// of squares and the scaling (rows up to WPR * kHeld * 256 columns).
+template <typename TX, typename TD, bool DELTA, bool VEC, int WPR>
+__global__ void __launch_bounds__(32 * kWarps, 3) fp8_rmsnorm_kernel(const __grid_constant__ Fp8RowsParams p) {
   __shared__ float part[kWarps];
   pdl_wait();
   pdl_launch_next();
+  constexpr int kStep = WPR * kUnit;  // columns between a warp's units
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wi = warp % WPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kWarps / WPR) + warp / WPR;
-  const bool live = row < p.m;
-  const int k = live ? static_cast<int>(p.k) : 0;
-  constexpr int kStep = WPR * kFp8Block;  // columns between a warp's blocks
-  const int64_t off = wi * kFp8Block + lane * 4;
+  const int off = wi * kUnit + lane * 8;
+  const int left0 = row < p.m ? static_cast<int>(p.k) - off : 0;  // columns from this lane's first element on
   const TX* x = static_cast<const TX*>(p.x) + row * p.ldx + off;
   const TD* d = DELTA ? static_cast<const TD*>(p.delta) + row * p.ldd + off : nullptr;
-  const int left0 = k - static_cast<int>(off);  // columns from this lane's first element on
-  float4 v[HELD];
+  Raw8<TX> rx[kHeld];
+  Raw8<TD> rd[DELTA ? kHeld : 1];
+#pragma unroll
+  for (int g = 0; g < kHeld; ++g) {
+    rx[g] = get8<VEC>(x + g * kStep, left0 - g * kStep);
+    if constexpr (DELTA) rd[g] = get8<VEC>(d + g * kStep, left0 - g * kStep);
+  }
+  Eight v[kHeld];
   float ss = 0.f;
-  auto fetch = [&](int c0) {  // blocks at columns c0 + off + kStep g
-    Raw4<TX> rx[HELD];
-    Raw4<TD> rd[HELD];
 #pragma unroll
-    for (int g = 0; g < HELD; ++g) {
-      rx[g] = get4<VEC>(x + c0 + g * kStep, left0 - c0 - g * kStep);
-      if (DELTA) rd[g] = get4<VEC>(d + c0 + g * kStep, left0 - c0 - g * kStep);
+  for (int g = 0; g < kHeld; ++g) {
+    v[g] = widen(rx[g]);
+    if constexpr (DELTA) {
+      const Eight e = widen(rd[g]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[g].v[i] += e.v[i];
     }
 #pragma unroll
-    for (int g = 0; g < HELD; ++g) {
-      v[g] = widen(rx[g]);
-      if (DELTA) {
-        const float4 e = widen(rd[g]);
-        v[g].x += e.x;
-        v[g].y += e.y;
-        v[g].z += e.z;
-        v[g].w += e.w;
-      }
-    }
-  };
-  for (int c0 = 0; c0 == 0 || (WIDE && c0 < k); c0 += HELD * kStep) {
-    fetch(c0);
-#pragma unroll
-    for (int g = 0; g < HELD; ++g) ss += v[g].x * v[g].x + v[g].y * v[g].y + v[g].z * v[g].z + v[g].w * v[g].w;
+    for (int i = 0; i < 8; ++i) ss += v[g].v[i] * v[g].v[i];
   }
   ss = warp_total(ss);
   if (WPR > 1) {
@@ -166,47 +205,90 @@ __global__ void __launch_bounds__(32 * kWarps, WIDE ? 2 : 4)
 #pragma unroll
     for (int i = 0; i < WPR; ++i) ss += part[warp / WPR * WPR + i];
   }
-  if (!live) return;
-  const float inv = 1.0f / sqrtf(ss / static_cast<float>(k) + p.eps);
+  if (row >= p.m) return;
+  const float inv = __frcp_rn(sqrtf(ss / static_cast<float>(p.k) + p.eps));
   TX* sum = DELTA ? static_cast<TX*>(p.sum) + row * p.ldsum + off : nullptr;
   uint8_t* codes = p.codes + row * p.ldc + off;
-  float* scales = p.scales + row * p.lds + wi + WPR * lane;
-  const float* wt = p.w + off;
-  for (int c0 = 0; c0 == 0 || (WIDE && c0 < k); c0 += HELD * kStep) {
-    if (WIDE) fetch(c0);
-    float mine = 0.f;
+  float* scales = p.scales + row * p.lds + off / kFp8Block;
 #pragma unroll
-    for (int g = 0; g < HELD; ++g) {
-      const int c = c0 + g * kStep, left = left0 - c;
-      if (left + lane * 4 <= 0) break;  // the whole block is past the row
-      const float4 w = widen(get4<VEC>(wt + c, left));
-      if (DELTA) put4<VEC>(sum + c, left, v[g]);
-      const float4 y = make_float4(v[g].x * inv * w.x, v[g].y * inv * w.y, v[g].z * inv * w.z, v[g].w * inv * w.w);
-      const float s = fp8_scale(warp_max_nan(max4_nan(y)));
-      if (lane == g) mine = s;
-      put_codes<VEC>(codes + c, left, codes4(y, fp8_factor(s)));
-    }
-    if (lane < HELD && left0 + lane * 4 > c0 + lane * kStep) scales[c0 / kFp8Block] = mine;
+  for (int g = 0; g < kHeld; ++g) {
+    const int left = left0 - g * kStep;
+    if (left + lane * 8 <= 0) break;  // the whole unit is past the row
+    if (DELTA) put8<VEC>(sum + g * kStep, left, v[g]);
+    const Eight w = widen(get8<VEC>(p.w + off + g * kStep, left));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[g].v[i] *= inv * w.v[i];
+    put_unit<VEC>(codes + g * kStep, scales + g * (kStep / kFp8Block), lane, left, v[g]);
   }
 }
 
-// One CTA per 128 x 128 block, 16 rows per warp held in registers.
-template <typename T>
+// A row wider than the registers of a CTA: read twice, the second time from L2.
+template <typename TX, typename TD, bool DELTA, bool VEC>
+__global__ void __launch_bounds__(32 * kWarps) fp8_rmsnorm_wide_kernel(const __grid_constant__ Fp8RowsParams p) {
+  __shared__ float part[kWarps];
+  pdl_wait();
+  pdl_launch_next();
+  constexpr int kStep = kWarps * kUnit;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int off = warp * kUnit + lane * 8, k = static_cast<int>(p.k);
+  const int64_t row = blockIdx.x;
+  const TX* x = static_cast<const TX*>(p.x) + row * p.ldx + off;
+  const TD* d = DELTA ? static_cast<const TD*>(p.delta) + row * p.ldd + off : nullptr;
+  auto value = [&](int c) {
+    Eight v = widen(get8<VEC>(x + c, k - off - c));
+    if constexpr (DELTA) {
+      const Eight e = widen(get8<VEC>(d + c, k - off - c));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v.v[i] += e.v[i];
+    }
+    return v;
+  };
+  float ss = 0.f;
+#pragma unroll 2
+  for (int c = 0; c < k; c += kStep) {
+    const Eight v = value(c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += v.v[i] * v.v[i];
+  }
+  ss = warp_total(ss);
+  if (lane == 0) part[warp] = ss;
+  __syncthreads();
+  ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) ss += part[i];
+  const float inv = __frcp_rn(sqrtf(ss / static_cast<float>(k) + p.eps));
+  TX* sum = DELTA ? static_cast<TX*>(p.sum) + row * p.ldsum + off : nullptr;
+#pragma unroll 2
+  for (int c = 0; c < k - warp * kUnit; c += kStep) {
+    const int left = k - off - c;
+    Eight v = value(c);
+    if (DELTA) put8<VEC>(sum + c, left, v);
+    const Eight w = widen(get8<VEC>(p.w + off + c, left));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.v[i] *= inv * w.v[i];
+    put_unit<VEC>(p.codes + row * p.ldc + off + c, p.scales + row * p.lds + (off + c) / kFp8Block, lane, left, v);
+  }
+}
+
+// One CTA per 128 x 128 block, eight elements of eight rows per thread.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * kWarps) fp8_weight_kernel(const __grid_constant__ Fp8RowsParams p, int kblocks) {
   __shared__ float part[kWarps];
   pdl_wait();
   pdl_launch_next();
-  constexpr int kRows = kFp8Block / kWarps;
+  constexpr int kTurns = kFp8Block / (2 * kWarps);  // a warp takes two rows at a time
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t nb = blockIdx.x / kblocks, kb = blockIdx.x % kblocks;
-  const int64_t row0 = nb * kFp8Block + warp * kRows, col = kb * kFp8Block + lane * 4, left = p.k - col;
+  const int64_t row0 = nb * kFp8Block + warp * 2 + (lane >> 4), col = kb * kFp8Block + (lane & 15) * 8;
+  const int left = static_cast<int>(p.k - col);
   const T* x = static_cast<const T*>(p.x) + row0 * p.ldx + col;
-  float4 v[kRows];
+  Raw8<T> v[kTurns];
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) v[r] = load4(x + r * p.ldx, row0 + r < p.m ? left : 0, p.vec_x);
+  for (int t = 0; t < kTurns; ++t)
+    v[t] = get8<VEC>(x + 2 * kWarps * t * p.ldx, row0 + 2 * kWarps * t < p.m ? left : 0);
   float a = 0.f;
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) a = max_nan(a, max4_nan(v[r]));
+  for (int t = 0; t < kTurns; ++t) a = max_nan(a, max_abs(widen(v[t])));
   a = warp_max_nan(a);
   if (lane == 0) part[warp] = a;
   __syncthreads();
@@ -215,8 +297,10 @@ __global__ void __launch_bounds__(32 * kWarps) fp8_weight_kernel(const __grid_co
   const float s = fp8_scale(a), f = fp8_factor(s);
   if (threadIdx.x == 0) p.scales[nb * p.lds + kb] = s;
 #pragma unroll
-  for (int r = 0; r < kRows; ++r)
-    if (row0 + r < p.m) store_codes4(p.codes + (row0 + r) * p.ldc + col, left, codes4(v[r], f));
+  for (int t = 0; t < kTurns; ++t) {
+    const int64_t row = row0 + 2 * kWarps * t;
+    if (row < p.m) put_codes8<VEC>(p.codes + row * p.ldc + col, left, widen(v[t]), f);
+  }
 }
 
 // Grid of at most 2^31 - 1 CTAs.
@@ -228,22 +312,22 @@ bool grid_of(int64_t n, dim3* g) {
 
 template <typename TX, typename TD, bool DELTA, bool VEC>
 cudaError_t rmsnorm(const Fp8RowsParams& p, cudaStream_t st) {
-  const int64_t kb = (p.k + kFp8Block - 1) / kFp8Block;
+  const int64_t units = (p.k + kUnit - 1) / kUnit;
   auto go = [&](auto kernel, int wpr) {
     dim3 grid;
     if (!grid_of((p.m + kWarps / wpr - 1) / (kWarps / wpr), &grid)) return cudaErrorInvalidValue;
     return launch_pdl(kernel, grid, dim3(32 * kWarps), 0, st, nullptr, 0, p);
   };
-  if (kb <= 6) return go(fp8_rmsnorm_kernel<TX, TD, DELTA, VEC, 1, 6, false>, 1);
-  if (kb <= 12) return go(fp8_rmsnorm_kernel<TX, TD, DELTA, VEC, 2, 6, false>, 2);
-  if (kb <= 24) return go(fp8_rmsnorm_kernel<TX, TD, DELTA, VEC, 4, 6, false>, 4);
-  if (kb <= 48) return go(fp8_rmsnorm_kernel<TX, TD, DELTA, VEC, 8, 6, false>, 8);
-  return go(fp8_rmsnorm_kernel<TX, TD, DELTA, VEC, 8, 8, true>, 8);
+  if (units <= kHeld) return go(fp8_rmsnorm_kernel<TX, TD, DELTA, VEC, 1>, 1);
+  if (units <= 2 * kHeld) return go(fp8_rmsnorm_kernel<TX, TD, DELTA, VEC, 2>, 2);
+  if (units <= 4 * kHeld) return go(fp8_rmsnorm_kernel<TX, TD, DELTA, VEC, 4>, 4);
+  if (units <= 8 * kHeld) return go(fp8_rmsnorm_kernel<TX, TD, DELTA, VEC, 8>, 8);
+  return go(fp8_rmsnorm_wide_kernel<TX, TD, DELTA, VEC>, 8);
 }
 
 template <typename TX, typename TD, bool DELTA>
 cudaError_t rmsnorm_v(const Fp8RowsParams& p, cudaStream_t st) {
-  const bool vec = p.vec_x && p.vec_w && (!DELTA || (p.vec_d && p.vec_s)) && p.k % 4 == 0;
+  const bool vec = p.vec_x && p.vec_w && (!DELTA || (p.vec_d && p.vec_s)) && p.k % 8 == 0;
   return vec ? rmsnorm<TX, TD, DELTA, true>(p, st) : rmsnorm<TX, TD, DELTA, false>(p, st);
 }
 
@@ -260,10 +344,10 @@ cudaError_t rmsnorm_d(int delta_type, const Fp8RowsParams& p, cudaStream_t st) {
 
 template <typename T>
 cudaError_t rows(const Fp8RowsParams& p, cudaStream_t st) {
-  const int64_t groups = (p.k + kRowsHeld * kFp8Block - 1) / (kRowsHeld * kFp8Block);
+  const int64_t groups = (p.k + kHeld * kUnit - 1) / (kHeld * kUnit);
   dim3 grid;
   if (groups > 0x7FFFFFFF || !grid_of((p.m * groups + kWarps - 1) / kWarps, &grid)) return cudaErrorInvalidValue;
-  auto kernel = p.vec_x && p.k % 4 == 0 ? fp8_rows_kernel<T, true> : fp8_rows_kernel<T, false>;
+  auto kernel = p.vec_x && p.k % 8 == 0 ? fp8_rows_kernel<T, true> : fp8_rows_kernel<T, false>;
   return launch_pdl(kernel, grid, dim3(32 * kWarps), 0, st, nullptr, 0, p, static_cast<int>(groups));
 }
 
@@ -272,7 +356,8 @@ cudaError_t weight(const Fp8RowsParams& p, cudaStream_t st) {
   const int64_t kb = (p.k + kFp8Block - 1) / kFp8Block, nb = (p.m + kFp8Block - 1) / kFp8Block;
   dim3 grid;
   if (kb > 0x7FFFFFFF || !grid_of(kb * nb, &grid)) return cudaErrorInvalidValue;
-  return launch_pdl(fp8_weight_kernel<T>, grid, dim3(32 * kWarps), 0, st, nullptr, 0, p, static_cast<int>(kb));
+  auto kernel = p.vec_x && p.k % 8 == 0 ? fp8_weight_kernel<T, true> : fp8_weight_kernel<T, false>;
+  return launch_pdl(kernel, grid, dim3(32 * kWarps), 0, st, nullptr, 0, p, static_cast<int>(kb));
 }
 
 }  // namespace

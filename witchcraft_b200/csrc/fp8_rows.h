@@ -14,7 +14,7 @@ struct Fp8RowsParams {
   float* scales;      // [m][lds]
   int64_t m, k, ldx, ldd, ldsum, ldc, lds;
   float eps;
-  bool vec_x, vec_d, vec_s, vec_w;  // rows aligned to four elements
+  bool vec_x, vec_d, vec_s, vec_w;  // rows aligned to eight elements
 };
 
 cudaError_t fp8_rows_launch(int x_type, Fp8RowsParams p, cudaStream_t st);
