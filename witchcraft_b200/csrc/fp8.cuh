@@ -34,6 +34,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
+// Largest magnitude of three, keeping a NaN.
+__device__ __forceinline__ float max_abs3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // max_nan over the warp, in every lane.
 __device__ __forceinline__ float warp_max_nan(float v) {
   float d;

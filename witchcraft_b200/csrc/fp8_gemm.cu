@@ -229,12 +229,25 @@ __device__ __forceinline__ bool sum_blocks(float (&acc)[32 * CHUNKS], Scales& sc
 
 // act(g) u, both activations in the form g / (1 + exp(-z)): z = g (SiLU), or
 // z = 2 sqrt(2 / pi) (g + 0.044715 g^3), since (1 + tanh(z / 2)) / 2 =
-// 1 / (1 + exp(-z)).  exp and the quotient are the fast f32 ones (a few ulp):
-// the 11-bit hardware tanh would show in the f32 scales of 8-bit rows.
-__device__ __forceinline__ float gate(float g, float u, int act) {
-  const float z = act == WC_ACT_SILU ? g : 1.5957691216f * (g + 0.044715f * g * g * g);
-  return g * __fdividef(1.0f, 1.0f + __expf(-z)) * u;
-}
+// 1 / (1 + exp(-z)).  So -z log2(e) = g (c1 + c3 g^2) with two constants, and
+// the exponential and the quotient are the hardware's f32 approximations (a
+// few ulp): its 11-bit tanh would show in the f32 scales of 8-bit rows.  g^2
+// is kept finite so that SiLU's c3 = 0 does not meet an infinity.
+struct Gate {
+  float c1, c3;
+  __device__ __forceinline__ explicit Gate(int act) {
+    constexpr float log2e = 1.4426950409f;
+    c1 = act == WC_ACT_SILU ? -log2e : -1.5957691216f * log2e;
+    c3 = act == WC_ACT_SILU ? 0.0f : -1.5957691216f * 0.044715f * log2e;
+  }
+  __device__ __forceinline__ float operator()(float g, float u) const {
+    const float z = g * __fmaf_rn(c3, fminf(g * g, 1e30f), c1);
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return g * r * u;
+  }
+};
 
 __device__ __forceinline__ void regs_for_epilogue() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
 __device__ __forceinline__ void regs_given_back() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
@@ -293,8 +306,10 @@ constexpr int kStages = 5;
 constexpr int kStageBytes = kABytes + 128 * kFp8Block;
 constexpr int kBoxBytes = 32 * 128;  // 32 rows x 128 bytes of results (or of the residual)
 constexpr int kOffOut = kStages * kStageBytes;
-constexpr int kOffAmax = kOffOut + 8 * 2 * kBoxBytes;  // two boxes per epilogue warp
-constexpr int kOffBar = kOffAmax + 2 * kRows * 4;
+constexpr int kOffBar = kOffOut + 8 * 2 * kBoxBytes;  // two boxes per epilogue warp
+// block maxima of 8-bit rows, in a second box: codes need only the first
+constexpr int kOffAmax = kOffOut + kBoxBytes;
+static_assert(2 * 2 * kRows * 4 <= kBoxBytes, "maxima of two tiles");
 constexpr int kSmem = 1024 + kOffBar + 256;
 static_assert(kSmem <= 232448, "dynamic shared memory per block");
 
@@ -380,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_for_epilogue();
     const int q = warp & 3, h = (warp >> 2) - 1;  // TMEM lane quarter, column half
     uint8_t* box = smem + kOffOut + (warp - 4) * 2 * kBoxBytes;
-    float* amax = reinterpret_cast<float*>(smem + kOffAmax);  // [half][row of the tile]
+    float* amax = reinterpret_cast<float*>(smem + kOffAmax);  // [tile parity][half][row of the tile]
     const uint32_t tlane = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * 128;
     const uint32_t empty0 = map_to_rank(&acc_empty[0], 0);
     // A tile's scales, the first block's on their way (past the last tile: the last one's).
@@ -406,6 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     Ring<kStages> ring;
+    uint32_t turn = 0;  // tiles of 8-bit rows so far
     bool ok = true;
     Scales sc = open_tile(tile0);
     for (int tile = tile0; tile < tiles && ok; tile += tile_step) {
@@ -429,37 +445,44 @@ __global__ void __launch_bounds__(kThreads, 1)
 
       const int row = row0 + lane;
       if constexpr (GATED) {
+        const Gate gate(p.act);
 #pragma unroll
-        for (int j = 0; j < 64; ++j) acc[j] = gate(acc[j], acc[64 + j], p.act);
+        for (int j = 0; j < 64; ++j) acc[j] = gate(acc[j], acc[64 + j]);
       }
       if constexpr (kCodes) {
         // The 64 results of this thread and those of the thread with the same
         // row in the other half are one block of 128.
         float a = 0.f;
 #pragma unroll
-        for (int j = 0; j < 64; ++j) a = max_nan(a, fabsf(acc[j]));
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // the maxima of the tile before have been read
-        amax[h * kRows + q * 32 + lane] = a;
+        for (int j = 0; j < 64; j += 2) a = max_abs3_nan(a, acc[j], acc[j + 1]);
+        float* shared = amax + (turn & 1) * 2 * kRows;  // the tile before may still be reading its own
+        ++turn;
+        shared[h * kRows + q * 32 + lane] = a;
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        const float os = fp8_scale(max_nan(a, amax[(h ^ 1) * kRows + q * 32 + lane])), fac = fp8_factor(os);
-        if (row < p.m) {
-          if (h == 0) p.out_scales[row * p.ldos + f0 / kFp8Block] = os;
-          uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.ldo + col0;
+        const float os = fp8_scale(max_nan(a, shared[(h ^ 1) * kRows + q * 32 + lane])), fac = fp8_factor(os);
+        if (h == 0 && row < p.m) p.out_scales[row * p.ldos + f0 / kFp8Block] = os;
+        // 32 rows x 64 codes by one TMA store (64-byte swizzle)
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {  // 16 codes
-            uint32_t w[4];
+        for (int c = 0; c < 4; ++c) {  // 16 codes
+          uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = pack_e4m3x4(acc[16 * c + 4 * e] * fac, acc[16 * c + 4 * e + 1] * fac, acc[16 * c + 4 * e + 2] * fac,
-                                 acc[16 * c + 4 * e + 3] * fac);
-            const int left = p.n - col0 - 16 * c;
-            if (left >= 16) {
-              *reinterpret_cast<uint4*>(o + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) store_codes4(o + 16 * c + 4 * e, left - 4 * e, w[e]);
-            }
-          }
+          for (int e = 0; e < 4; ++e)
+            w[e] = pack_e4m3x4(acc[16 * c + 4 * e] * fac, acc[16 * c + 4 * e + 1] * fac, acc[16 * c + 4 * e + 2] * fac,
+                               acc[16 * c + 4 * e + 3] * fac);
+          *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (col0 < p.n && row0 < p.m)
+            asm volatile(
+                "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                    reinterpret_cast<uint64_t>(&tmOut)),
+                "r"(smem_u32(box)), "r"(col0), "r"(row0)
+                : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
       } else {
         if (boxes) {
@@ -719,11 +742,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         // lane: features 4 lane .. 4 lane + 3 of the tile's 128
         const int c = (lane >> 4) * 32 + (lane & 15);
         const float4 g = total(r, c), u = total(r, c + 16);
-        const float4 v = make_float4(gate(g.x, u.x, p.act), gate(g.y, u.y, p.act), gate(g.z, u.z, p.act),
-                                     gate(g.w, u.w, p.act));
+        const Gate gate(p.act);
+        const float4 v = make_float4(gate(g.x, u.x), gate(g.y, u.y), gate(g.z, u.z), gate(g.w, u.w));
         const int col = f0 + lane * 4;
         if constexpr (kCodes) {
-          const float a = max_nan(max_nan(fabsf(v.x), fabsf(v.y)), max_nan(fabsf(v.z), fabsf(v.w)));
+          const float a = max_abs3_nan(max_abs3_nan(v.x, v.y, v.z), v.w, v.w);
           const float sc = fp8_scale(warp_max_nan(a)), fac = fp8_factor(sc);
           if (lane == 0) p.out_scales[row * p.ldos + f0 / kFp8Block] = sc;
           store_codes4(static_cast<uint8_t*>(p.out) + row * p.ldo + col, p.n - col,
@@ -781,18 +804,20 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// Codes [rows][ld] of which k columns are read: box 128 x box_rows, 128-byte
-// swizzle, zeros outside.
-bool codes_map(CUtensorMap* m, const uint8_t* ptr, int64_t rows, int64_t k, int64_t ld, uint32_t box_rows) {
+// Codes [rows][ld] of which k columns are meant: box `box_cols` (128 or 64)
+// x box_rows, swizzled over the box's width, zeros outside.
+bool codes_map(CUtensorMap* m, const uint8_t* ptr, int64_t rows, int64_t k, int64_t ld, uint32_t box_rows,
+               uint32_t box_cols = kFp8Block) {
   const EncodeTiledFn enc = encode_fn();
   if (!enc) return false;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
-  cuuint32_t box[2] = {kFp8Block, box_rows};
+  cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t es[2] = {1, 1};
   return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(ptr), dims, strides, box, es,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+             CU_TENSOR_MAP_INTERLEAVE_NONE,
+             box_cols == kFp8Block ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Results or residual [rows][ld]: boxes of 32 rows x 128 bytes, 128-byte swizzle.
@@ -854,7 +879,9 @@ cudaError_t launch_pair(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
   // results by TMA boxes where rows (and the residual's) start at multiples of 16 bytes
   CUtensorMap to = ta, tr = ta;
   bool boxes = false;
-  if constexpr (sizeof(OutT) > 1) {
+  if constexpr (sizeof(OutT) == 1) {
+    if (!codes_map(&to, static_cast<const uint8_t*>(p.out), p.m, p.n, p.ldo, 32, 64)) return cudaErrorInvalidValue;
+  } else {
     boxes = p.box_o && (!p.residual || p.box_r);
     if (boxes && (!values_map<OutT>(&to, p.out, p.m, p.n, p.ldo) ||
                   (p.residual && !values_map<OutT>(&tr, p.residual, p.m, p.n, p.ldr))))

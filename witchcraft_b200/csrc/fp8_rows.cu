@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kUnit = 2 * kFp8Block;  // columns a warp takes at a time
-constexpr int kHeld = 4;              // units of a row that a warp loads at once
+constexpr int kHeld = 3;              // units of a row that a warp loads at once
 
 struct Eight {
   float v[8];
@@ -72,7 +72,9 @@ __device__ __forceinline__ Eight widen(const Raw8<__nv_bfloat16>& r) {
   }
   return e;
 }
-// Eight elements at p, of which `left` belong to the row; zeros past it.
+// Eight elements at p, of which `left` belong to the row; zeros past it.  Each
+// is read once: marked to be evicted first (norm m = 16384, k = 768: 30.2 ->
+// 28.8 us).
 template <bool VEC, typename T>
 __device__ __forceinline__ Raw8<T> get8(const T* p, int left) {
   Raw8<T> r;
@@ -80,15 +82,15 @@ __device__ __forceinline__ Raw8<T> get8(const T* p, int left) {
     if constexpr (VEC) {
       r.a = r.b = make_float4(0.f, 0.f, 0.f, 0.f);
       if (left > 0) {
-        r.a = reinterpret_cast<const float4*>(p)[0];
-        r.b = reinterpret_cast<const float4*>(p)[1];
+        r.a = __ldcs(reinterpret_cast<const float4*>(p));
+        r.b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
       }
     } else {
       r.a = load4(p, left, false);
       r.b = load4(p + 4, static_cast<int64_t>(left) - 4, false);
     }
   } else if constexpr (VEC) {
-    r.u = left > 0 ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
+    r.u = left > 0 ? __ldcs(reinterpret_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
   } else {
     const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
     uint32_t w[4];
