@@ -275,14 +275,16 @@ struct Pack<float> {
     v[3] += __uint_as_float(r.w);
   }
 };
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) { return pack_f16x2(a, b); }
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 template <typename T>
 struct Pack {
   static constexpr int kN = 8;
   static __device__ __forceinline__ uint4 make(const float* v) {
-    T e[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
-    return *reinterpret_cast<const uint4*>(e);
+    return make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
   }
   static __device__ __forceinline__ void add(float* v, uint4 r) {
     const T* e = reinterpret_cast<const T*>(&r);
@@ -486,43 +488,51 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         if (boxes) {
-          // One box at a time: converted into shared memory (128-byte swizzle)
-          // and written by one TMA store, which clips what lies outside.
+          // Two boxes at a time: converted into shared memory (128-byte
+          // swizzle) and written by TMA stores, which clip what lies outside.
+          constexpr int kN = Pack<OutT>::kN, kPair = kBoxes < 2 ? 1 : 2;
 #pragma unroll
-          for (int c = 0; c < kBoxes; ++c) {
-            uint8_t* b = box + (c & 1) * kBoxBytes;
-            const int x = col0 + c * kBoxCols;
-            const bool inside = x < p.n && row0 < p.m;
+          for (int c0 = 0; c0 < kBoxes; c0 += kPair) {
             if (res_boxes) {
-              if (inside) {
-                if (!mbar_wait(&res_bar[c & 1], (res_phase >> (c & 1)) & 1, status)) ok = false;
-                res_phase ^= 1u << (c & 1);
-              }
+              bool there = true;
+#pragma unroll
+              for (int b = 0; b < kPair; ++b)
+                if (col0 + (c0 + b) * kBoxCols < p.n && row0 < p.m) {
+                  there = there && mbar_wait(&res_bar[b], (res_phase >> b) & 1, status);
+                  res_phase ^= 1u << b;
+                }
+              ok = __all_sync(0xFFFFFFFFu, there) && ok;
             } else {
-              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
               __syncwarp();
             }
-            constexpr int kN = Pack<OutT>::kN;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              uint4* at = reinterpret_cast<uint4*>(b + lane * 128 + ((k ^ (lane & 7)) << 4));
-              float* v = acc + c * kBoxCols + k * kN;
-              if (res_boxes && inside) Pack<OutT>::add(v, *at);
-              *at = Pack<OutT>::make(v);
-            }
+            for (int b = 0; b < kPair; ++b)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                uint4* at = reinterpret_cast<uint4*>(box + b * kBoxBytes + lane * 128 + ((k ^ (lane & 7)) << 4));
+                float* v = acc + (c0 + b) * kBoxCols + k * kN;
+                if (res_boxes) Pack<OutT>::add(v, *at);
+                *at = Pack<OutT>::make(v);
+              }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              if (inside)
-                asm volatile(
-                    "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
-                        reinterpret_cast<uint64_t>(&tmOut)),
-                    "r"(smem_u32(b)), "r"(x), "r"(row0)
-                    : "memory");
+#pragma unroll
+              for (int b = 0; b < kPair; ++b) {
+                const int x = col0 + (c0 + b) * kBoxCols;
+                if (x < p.n && row0 < p.m)
+                  asm volatile(
+                      "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                          reinterpret_cast<uint64_t>(&tmOut)),
+                      "r"(smem_u32(box + b * kBoxBytes)), "r"(x), "r"(row0)
+                      : "memory");
+              }
               asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-              if (kBoxes > 2 && res_boxes && c + 2 < kBoxes) {
+              if (kBoxes > 2 && res_boxes && c0 + 2 < kBoxes) {
                 asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                fetch_residual(c & 1, x + 2 * kBoxCols, row0);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) fetch_residual(b, col0 + (c0 + 2 + b) * kBoxCols, row0);
               }
             }
           }
