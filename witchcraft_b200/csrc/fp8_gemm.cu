@@ -78,19 +78,20 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // The MMA warp's loop over `steps` blocks: STAGES operand stages of
-// STAGE_BYTES (A, then B) and two partials of BN columns.  The whole warp
+// STAGE_BYTES (A, then B) and BUFS partials of BN columns.  The whole warp
 // runs it and one lane issues, so that descriptors stay in uniform registers:
 // the warp shares its scheduler with two epilogue warps that are busy with
 // multiply-adds, and every instruction in this loop is slow.
-template <bool PAIR, int STAGES, int STAGE_BYTES, int BN, typename Commit>
+template <bool PAIR, int STAGES, int STAGE_BYTES, int BUFS, int BN, typename Commit>
 __device__ __forceinline__ void mma_loop(uint32_t tmem, uint32_t idesc, uint32_t smem, uint64_t* full, uint64_t* done,
                                          uint64_t* acc_empty, uint32_t steps, uint32_t* status, Commit commit) {
   const uint64_t a0 = sw128_kmajor_desc(smem), b0 = sw128_kmajor_desc(smem + kABytes);
   uint32_t s = 0, round = 0;
 #pragma unroll 1
   for (uint32_t i = 0; i < steps; ++i) {
-    const uint32_t buf = i & 1;
-    const bool ok = mbar_wait(&full[s], round & 1, status) && mbar_wait(&acc_empty[buf], ((i >> 1) & 1) ^ 1, status);
+    const uint32_t buf = i % BUFS;
+    const bool ok =
+        mbar_wait(&full[s], round & 1, status) && mbar_wait(&acc_empty[buf], ((i / BUFS) & 1) ^ 1, status);
     if (!__all_sync(0xFFFFFFFFu, ok)) return;  // one way out for the whole warp
     tc_fence_after();
     const uint64_t a = a0 + s * (STAGE_BYTES >> 4), b = b0 + s * (STAGE_BYTES >> 4);
@@ -182,15 +183,15 @@ struct Ring {
 };
 
 // acc[] = sum over `blocks` (>= 1) blocks, `step` apart, of scale * partial for
-// this thread's row and 32 CHUNKS columns (taddr of partial 0; partial 1 lies
-// BN columns on).  sc holds the first block's scales.  The columns come 32 at
+// this thread's row and 32 CHUNKS columns (taddr of partial 0; the others lie
+// BN columns apart).  sc holds the first block's scales.  The columns come 32 at
 // a time, the next 32 loading while these are added.  The multiply-adds are
 // scalar: the packed form needs register pairs that a TMEM load's results have
 // to be moved into.  What matters most here is that nothing spills: keeping
 // the next block's first columns in flight across the loop's end made the
 // whole product twice as slow.  `read(buf)` once a partial is in registers.
 // False if a wait ran out.
-template <bool GATED, int CHUNKS, int STAGES, int BN, typename Read>
+template <bool GATED, int CHUNKS, int STAGES, int BUFS, int BN, typename Read>
 __device__ __forceinline__ bool sum_blocks(float (&acc)[32 * CHUNKS], Scales& sc, int blocks, int step, uint32_t taddr,
                                            uint64_t* done, Ring<STAGES>& ring, uint32_t* status, Read read) {
   static_assert(CHUNKS == 2 || CHUNKS == 4, "two register sets");
@@ -203,7 +204,7 @@ __device__ __forceinline__ bool sum_blocks(float (&acc)[32 * CHUNKS], Scales& sc
     if (left > 1) fetch_scales<GATED>(sc, step);
     if (!__all_sync(0xFFFFFFFFu, mbar_wait(&done[ring.stage], ring.parity, status))) return false;
     tc_fence_after();
-    const uint32_t at = taddr + (ring.i & 1) * BN;
+    const uint32_t at = taddr + ring.i % BUFS * BN;
     auto add = [&](int c) {
       const float s = 2 * c < CHUNKS ? s0 : s1;
 #pragma unroll
@@ -218,7 +219,7 @@ __device__ __forceinline__ bool sum_blocks(float (&acc)[32 * CHUNKS], Scales& sc
       } else {
         tc_fence_before();
     __syncwarp();
-    read(ring.i & 1);
+    read(ring.i % BUFS);
       }
       add(c);
     }
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1 && rank == 0) {
       constexpr uint32_t idesc = idesc_e4m3_f32(2 * kRows, kBN);
       const int mine = tiles > tile0 ? (tiles - tile0 + tile_step - 1) / tile_step : 0;
-      mma_loop<true, kStages, kStageBytes, kBN>(tmem_base, idesc, smem_u32(smem), full, done, acc_empty,
+      mma_loop<true, kStages, kStageBytes, 2, kBN>(tmem_base, idesc, smem_u32(smem), full, done, acc_empty,
                                                 static_cast<uint32_t>(mine) * kblocks,
                                                 status, [](uint64_t* b) { tc_commit_pair(b); });
     }
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fetch_residual(1, col0 + kBoxCols, row0);
       }
       float acc[128];
-      ok = sum_blocks<GATED, 4, kStages, kBN>(
+      ok = sum_blocks<GATED, 4, kStages, 2, kBN>(
           acc, sc, kblocks, 1, tlane, done, ring, status,
           [&](uint32_t buf) {
             if (lane == 0) mbar_arrive_remote(empty0 + buf * 8);
@@ -597,6 +598,7 @@ template <int BN>
 struct Plan {
   static constexpr int kStages = BN == 256 ? 4 : 6;
   static constexpr int kStageBytes = kABytes + BN * kFp8Block;
+  static constexpr int kBufs = static_cast<int>(kTmemCols) / BN;  // partials
   static constexpr int kOffBar = kStages * kStageBytes;
   static constexpr int kSmem = 1024 + kOffBar + 256;
   static_assert(kSmem <= 232448, "dynamic shared memory per block");
@@ -632,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + PL::kOffBar);
   uint64_t* done = full + PL::kStages;  // MMA done: stage free, partial ready
   uint64_t* acc_empty = done + PL::kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + PL::kBufs);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   uint32_t* status = p.status ? p.status : &g_fp8_status;
 
@@ -649,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&full[i], 1);
       mbar_init(&done[i], 1);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&acc_empty[i], epi_warps);
+    for (int i = 0; i < PL::kBufs; ++i) mbar_init(&acc_empty[i], epi_warps);
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmW);
@@ -685,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) drain_loads(full, PL::kStages, i, status);
     } else if (warp == 1) {
       constexpr uint32_t idesc = idesc_e4m3_f32(kRows, BN);
-      mma_loop<false, PL::kStages, PL::kStageBytes, BN>(
+      mma_loop<false, PL::kStages, PL::kStageBytes, PL::kBufs, BN>(
           tmem_base, idesc, smem_u32(smem), full, done, acc_empty,
           (kblocks - rank + split - 1) / split, status, [](uint64_t* b) { tc_commit(b); });
     }
@@ -701,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float acc[32 * kChunks];
       Ring<PL::kStages> ring;
       fetch_scales<GATED>(sc, split);
-      sum_blocks<GATED, kChunks, PL::kStages, BN>(
+      sum_blocks<GATED, kChunks, PL::kStages, PL::kBufs, BN>(
           acc, sc, blocks, split, tlane, done, ring, status,
           [&](uint32_t buf) {
             if (lane == 0) mbar_arrive(&acc_empty[buf]);

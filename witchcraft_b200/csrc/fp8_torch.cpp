@@ -83,12 +83,20 @@ int64_t codes_ld(const Tensor& t) {
 Tensor empty(int64_t r, int64_t c, at::ScalarType type, c10::Device device) {
   return at::empty({r, c}, at::TensorOptions().dtype(type).device(device));
 }
-Tensor empty_codes(int64_t r, int64_t c, c10::Device device) {
-  const int64_t wide = (c + 15) / 16 * 16;
-  Tensor t = empty(r, wide, at::kFloat8_e4m3fn, device);
-  return wide == c ? t : t.narrow(1, 0, c);
+// Codes [r][c] and scales [sr][ceil(c / 128)] in one allocation (an allocation
+// costs about as much as a launch): two tensors over one storage.
+std::tuple<Tensor, Tensor> empty_quantized(int64_t r, int64_t c, int64_t sr, c10::Device device) {
+  const int64_t wide = (c + 15) / 16 * 16, kb = blocks(c), offset = (r * wide + 255) / 256 * 64;  // in floats
+  const Tensor buf = at::empty({4 * (offset + sr * kb)}, at::TensorOptions().dtype(at::kByte).device(device));
+  auto over = [&](at::ScalarType type, int64_t at0, int64_t rows, int64_t cols, int64_t ld) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(),
+                                                        c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(at0);
+    t.unsafeGetTensorImpl()->set_sizes_and_strides(c10::IntArrayRef{rows, cols}, c10::IntArrayRef{ld, 1});
+    return t;
+  };
+  return {over(at::kFloat8_e4m3fn, 0, r, c, wide), over(at::kFloat, offset, sr, kb, kb)};
 }
-Tensor empty_scales(int64_t r, int64_t k, c10::Device device) { return empty(r, blocks(k), at::kFloat, device); }
 
 float* floats(const Tensor& t) { return static_cast<float*>(t.data_ptr()); }
 
@@ -110,7 +118,7 @@ Pair quantize(const Tensor& x) {
   columns(x, "x");
   const int64_t m = x.size(0), k = x.size(1);
   const c10::cuda::CUDAGuard guard(x.device());
-  Tensor codes = empty_codes(m, k, x.device()), scales = empty_scales(m, k, x.device());
+  auto [codes, scales] = empty_quantized(m, k, m, x.device());
   if (m)
     check(api.rows(x.data_ptr(), code, m, k, ld(x), codes.data_ptr(), codes_ld(codes), floats(scales), scales.size(1),
                    stream_of(x)));
@@ -122,7 +130,7 @@ Pair quantize_weight(const Tensor& w) {
   const int64_t n = w.size(0), k = w.size(1);
   if (n < 1 || k < 1) refuse("w is empty");
   const c10::cuda::CUDAGuard guard(w.device());
-  Tensor codes = empty_codes(n, k, w.device()), scales = empty_scales(blocks(n), k, w.device());
+  auto [codes, scales] = empty_quantized(n, k, blocks(n), w.device());
   check(api.weight(w.data_ptr(), code, n, k, ld(w), codes.data_ptr(), codes_ld(codes), floats(scales), scales.size(1),
                    stream_of(w)));
   return {codes, scales};
@@ -149,7 +157,7 @@ py::tuple rmsnorm(const Tensor& x, const Tensor& weight, double eps, const std::
   }
   const c10::cuda::CUDAGuard guard(x.device());
   Tensor sum = !delta ? Tensor() : out ? *out : empty(m, k, x.scalar_type(), x.device());
-  Tensor codes = empty_codes(m, k, x.device()), scales = empty_scales(m, k, x.device());
+  auto [codes, scales] = empty_quantized(m, k, m, x.device());
   if (m)
     check(api.rmsnorm(x.data_ptr(), code, ld(x), delta ? delta->data_ptr() : nullptr, dcode, delta ? ld(*delta) : 0,
                       delta ? sum.data_ptr() : nullptr, delta ? ld(sum) : 0, floats(weight), m, k,
@@ -206,8 +214,11 @@ py::object gated_matmul(const Tensor& a, const Tensor& a_scales, const Tensor& g
   if (code < 0)
     refuse(std::string("out_dtype must be None, float32, float16 or bfloat16, not ") + c10::toString(*out_dtype));
   const c10::cuda::CUDAGuard guard(a.device());
-  Tensor y = out_dtype ? empty(m, n, *out_dtype, a.device()) : empty_codes(m, n, a.device());
-  Tensor scales = out_dtype ? Tensor() : empty_scales(m, n, a.device());
+  Tensor y, scales;
+  if (out_dtype)
+    y = empty(m, n, *out_dtype, a.device());
+  else
+    std::tie(y, scales) = empty_quantized(m, n, m, a.device());
   if (m)
     check(api.gated(a.data_ptr(), codes_ld(a), floats(a_scales), ld(a_scales), m, k, gate.data_ptr(), codes_ld(gate),
                     floats(gate_scales), ld(gate_scales), up.data_ptr(), codes_ld(up), floats(up_scales),
