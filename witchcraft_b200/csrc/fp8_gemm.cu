@@ -82,10 +82,10 @@ __device__ __forceinline__ bool elect_one() {
 // runs it and one lane issues, so that descriptors stay in uniform registers:
 // the warp shares its scheduler with two epilogue warps that are busy with
 // multiply-adds, and every instruction in this loop is slow.
-template <bool PAIR, int STAGES, int STAGE_BYTES, int BUFS, int BN, typename Commit>
+template <bool PAIR, int STAGES, int STAGE_BYTES, int B_OFFSET, int BUFS, int BN, typename Commit>
 __device__ __forceinline__ void mma_loop(uint32_t tmem, uint32_t idesc, uint32_t smem, uint64_t* full, uint64_t* done,
                                          uint64_t* acc_empty, uint32_t steps, uint32_t* status, Commit commit) {
-  const uint64_t a0 = sw128_kmajor_desc(smem), b0 = sw128_kmajor_desc(smem + kABytes);
+  const uint64_t a0 = sw128_kmajor_desc(smem), b0 = sw128_kmajor_desc(smem + B_OFFSET);
   uint32_t s = 0, round = 0;
 #pragma unroll 1
   for (uint32_t i = 0; i < steps; ++i) {
@@ -134,7 +134,8 @@ __device__ __forceinline__ void tmem_ld32_wait(uint32_t (&r)[32]) {
 }
 
 // The scales of one thread's row and columns, fetched one block ahead of
-// their use.  The loads are volatile, or the compiler moves them down to it.
+// their use.  The loads are volatile, or the compiler moves them down to it;
+// the first one brings the next 64 scales of its row into L2.
 // Rows and columns outside the matrix use the last ones' scales (their results
 // are not stored).
 struct Scales {
@@ -143,7 +144,7 @@ struct Scales {
 };
 __device__ __forceinline__ float load_ahead(const float* p) {
   float v;
-  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  asm volatile("ld.global.nc.L2::256B.f32 %0, [%1];" : "=f"(v) : "l"(p));
   return v;
 }
 template <bool GATED>
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1 && rank == 0) {
       constexpr uint32_t idesc = idesc_e4m3_f32(2 * kRows, kBN);
       const int mine = tiles > tile0 ? (tiles - tile0 + tile_step - 1) / tile_step : 0;
-      mma_loop<true, kStages, kStageBytes, 2, kBN>(tmem_base, idesc, smem_u32(smem), full, done, acc_empty,
+      mma_loop<true, kStages, kStageBytes, kABytes, 2, kBN>(tmem_base, idesc, smem_u32(smem), full, done, acc_empty,
                                                 static_cast<uint32_t>(mine) * kblocks,
                                                 status, [](uint64_t* b) { tc_commit_pair(b); });
     }
@@ -594,15 +595,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 // warp reduction).  Rows past m are neither loaded nor read back.
 namespace tile {
 
-template <int BN>
+// A_ROWS: rows of A that a stage has room for.  With few rows the weights are
+// what streams, and the room goes to more stages: a load from DRAM takes about
+// 1.5 us, so 96 KB in flight are 64 GB/s an SM.  (The MMA still reads 128 rows:
+// what follows A in the stage fills the lanes that nothing reads.)
+template <int BN, int A_ROWS>
 struct Plan {
-  static constexpr int kStages = BN == 256 ? 4 : 6;
-  static constexpr int kStageBytes = kABytes + BN * kFp8Block;
+  static constexpr int kA = A_ROWS * kFp8Block;
+  static constexpr int kStageBytes = kA + BN * kFp8Block;
+  static constexpr int kStages = (232448 - 1024 - 512) / kStageBytes < 12 ? (232448 - 1024 - 512) / kStageBytes : 12;
   static constexpr int kBufs = static_cast<int>(kTmemCols) / BN;  // partials
   static constexpr int kOffBar = kStages * kStageBytes;
-  static constexpr int kSmem = 1024 + kOffBar + 256;
+  static constexpr int kSmem = 1024 + kOffBar + 512;
   static_assert(kSmem <= 232448, "dynamic shared memory per block");
-  static_assert(kRows * BN * 4 <= kOffBar, "the sums fit over the operand stages");
+  static_assert(A_ROWS * BN * 4 <= kOffBar, "the sums fit over the operand stages");
+  static_assert(kStageBytes % 1024 == 0 && BN * kFp8Block >= kABytes - kA, "A's 128 rows stay inside the stage");
 };
 
 // Byte offset of the 16-byte chunk c of row r of the sums (conflict-free both
@@ -620,12 +627,12 @@ __device__ __forceinline__ float4 load_cluster(uint32_t addr) {
   return v;
 }
 
-template <bool GATED, typename OutT, int BN>
+template <bool GATED, typename OutT, int BN, int A_ROWS>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                     const __grid_constant__ CUtensorMap tmU, const __grid_constant__ Fp8GemmParams p, int split,
                     int a_rows) {
-  using PL = Plan<BN>;
+  using PL = Plan<BN, A_ROWS>;
   constexpr bool kCodes = sizeof(OutT) == 1;
   constexpr int kChunks = BN / 64;  // 32-column chunks of a thread's half
   static_assert(!GATED || BN == 256, "the gated product needs 128 features of both weights");
@@ -681,13 +688,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_2d(sa, &tmA, &full[s], kb * kFp8Block, m0);
 #pragma unroll
         for (int c = 0; c < BN / 64; ++c)  // 64 weight rows each
-          tma_load_2d(sa + kABytes + c * 64 * kFp8Block, GATED && (c & 1) ? &tmU : &tmW, &full[s], kb * kFp8Block,
+          tma_load_2d(sa + PL::kA + c * 64 * kFp8Block, GATED && (c & 1) ? &tmU : &tmW, &full[s], kb * kFp8Block,
                       GATED ? f0 + (c >> 1) * 64 : f0 + c * 64);
       }
       if (!ok) drain_loads(full, PL::kStages, i, status);
     } else if (warp == 1) {
       constexpr uint32_t idesc = idesc_e4m3_f32(kRows, BN);
-      mma_loop<false, PL::kStages, PL::kStageBytes, PL::kBufs, BN>(
+      mma_loop<false, PL::kStages, PL::kStageBytes, PL::kA, PL::kBufs, BN>(
           tmem_base, idesc, smem_u32(smem), full, done, acc_empty,
           (kblocks - rank + split - 1) / split, status, [](uint64_t* b) { tc_commit(b); });
     }
@@ -904,13 +911,14 @@ cudaError_t launch_pair(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
                     boxes);
 }
 
-template <bool GATED, typename OutT, int BN>
+template <bool GATED, typename OutT, int BN, int A_ROWS>
 cudaError_t launch_tile(const Fp8GemmParams& p, int split, cudaStream_t st) {
-  constexpr auto kernel = tile::fp8_tile_kernel<GATED, OutT, BN>;
-  cudaError_t e = allow_smem<kernel>(tile::Plan<BN>::kSmem);
+  constexpr auto kernel = tile::fp8_tile_kernel<GATED, OutT, BN, A_ROWS>;
+  constexpr int kSmem = tile::Plan<BN, A_ROWS>::kSmem;
+  cudaError_t e = allow_smem<kernel>(kSmem);
   if (e != cudaSuccess) return e;
   // rows of a box of A: as many as there are, in steps of the swizzle's eight
-  const int a_rows = std::min(kRows, (p.m + 7) / 8 * 8);
+  const int a_rows = std::min(A_ROWS, (p.m + 7) / 8 * 8);
   CUtensorMap ta, tw, tu;
   if (!codes_map(&ta, p.a, p.m, p.k, p.lda, a_rows) || !codes_map(&tw, p.w, p.n, p.k, p.ldw, 64) ||
       !codes_map(&tu, GATED ? p.up : p.w, p.n, p.k, GATED ? p.ldup : p.ldw, 64))
@@ -919,9 +927,13 @@ cudaError_t launch_tile(const Fp8GemmParams& p, int split, cudaStream_t st) {
   const int64_t tiles = static_cast<int64_t>((p.m + kRows - 1) / kRows) * ((p.n + kFeat - 1) / kFeat);
   if (tiles * split > 0x7FFFFFFF) return cudaErrorInvalidValue;
   const cudaLaunchAttribute attr = cluster_of(split);
-  return launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * split)), dim3(kThreads), tile::Plan<BN>::kSmem, st,
-                    &attr, split > 1 ? 1 : 0, ta, tw, tu, p, split, a_rows);
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * split)), dim3(kThreads), kSmem, st, &attr,
+                    split > 1 ? 1 : 0, ta, tw, tu, p, split, a_rows);
 }
+
+struct Cost {  // us
+  float tile, tile_rows, block, join, pair_start, pair_round, pair_block;
+};
 
 template <bool GATED, typename OutT>
 cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
@@ -929,16 +941,36 @@ cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
   constexpr int kFeat = 128;  // output columns of a single tile
   const int64_t kblocks = (static_cast<int64_t>(p.k) + kFp8Block - 1) / kFp8Block;
   const int64_t tiles = static_cast<int64_t>((p.m + kRows - 1) / kRows) * ((p.n + kFeat - 1) / kFeat);
-  if (tiles > 2 * num_sms) return launch_pair<GATED, OutT>(p, num_sms, st);
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= num_sms && split * 2 <= kblocks) split *= 2;
-#ifdef WC_FP8_SWEEP
-  if (const char* f = getenv("WC_FP8_FORCE")) {
-    if (atoi(f) == 0) return launch_pair<GATED, OutT>(p, num_sms, st);
-    split = std::min<int>(atoi(f), kblocks);
+  // Which kernel, and how many CTAs share a tile's K: whichever should end
+  // first by what was measured (us, inputs from DRAM).  A single tile costs a
+  // start and an end that grow with its rows, and its blocks one after the
+  // other; a join over a cluster costs extra; more tiles than SMs go in rounds.
+  // A pair's round is cheaper per element but starts slower, and rows off the
+  // 16-byte boundary cost it an element-wise way out.  Measured with 768 <= k <=
+  // 8192, 1 <= m <= 4096; at m = 128, k = 768, n = 2304: 6.1 / 6.8 / 5.6 / 6.5 us
+  // with 1, 2, 4, 8 CTAs a tile and 6.8 on pairs.
+  const Cost c = GATED ? Cost{2.8f, 4.2f, 0.46f, 0.6f, 2.8f, 1.8f, 0.45f} : Cost{2.05f, 1.95f, 0.32f, 0.65f, 4.0f, 1.0f, 0.42f};
+  const float rows = static_cast<float>(std::min<int64_t>(p.m, kRows)) / kRows;
+  constexpr int kPairFeat = GATED ? 128 : 256;
+  const int64_t pairs = static_cast<int64_t>((p.m + 2 * kRows - 1) / (2 * kRows)) * ((p.n + kPairFeat - 1) / kPairFeat);
+  const bool off = sizeof(OutT) > 1 && !(p.box_o && (!p.residual || p.box_r));
+  float best = c.pair_start + static_cast<float>((pairs + clusters_of(num_sms) - 1) / clusters_of(num_sms)) *
+                                  (c.pair_round + c.pair_block * kblocks + (off ? 3.5f : 0.0f));
+  int split = 0;  // pairs
+  for (int s = 1; s <= 8 && s <= kblocks; s *= 2) {
+    const float rounds = static_cast<float>((tiles * s + num_sms - 1) / num_sms);
+    const float t = rounds * (c.tile + c.tile_rows * rows + c.block * static_cast<float>((kblocks + s - 1) / s) +
+                              (s > 1 ? c.join : 0.0f));
+    if (t < best) {
+      best = t;
+      split = s;
+    }
   }
+#ifdef WC_FP8_SWEEP
+  if (const char* f = getenv("WC_FP8_FORCE")) split = std::min<int>(atoi(f), kblocks);
 #endif
-  return launch_tile<GATED, OutT, BN>(p, split, st);
+  if (split == 0) return launch_pair<GATED, OutT>(p, num_sms, st);
+  return p.m <= 32 ? launch_tile<GATED, OutT, BN, 32>(p, split, st) : launch_tile<GATED, OutT, BN, kRows>(p, split, st);
 }
 
 }  // namespace
