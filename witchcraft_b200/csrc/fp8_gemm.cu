@@ -306,37 +306,51 @@ struct Pack {
 namespace pair {
 
 constexpr int kBN = 256;
-constexpr int kStages = 5;
 constexpr int kStageBytes = kABytes + 128 * kFp8Block;
 constexpr int kBoxBytes = 32 * 128;  // 32 rows x 128 bytes of results (or of the residual)
-constexpr int kOffOut = kStages * kStageBytes;
-constexpr int kOffBar = kOffOut + 8 * 2 * kBoxBytes;  // two boxes per epilogue warp
-// block maxima of 8-bit rows, in a second box: codes need only the first
-constexpr int kOffAmax = kOffOut + kBoxBytes;
-static_assert(2 * 2 * kRows * 4 <= kBoxBytes, "maxima of two tiles");
-constexpr int kSmem = 1024 + kOffBar + 256;
-static_assert(kSmem <= 232448, "dynamic shared memory per block");
+
+// Shared memory: operand stages, then boxes of results for each epilogue warp
+// (a warp's results are four boxes of f32 or two of 16-bit values).
+template <bool GATED, typename OutT>
+struct Plan {
+  static constexpr bool kCodes = sizeof(OutT) == 1;  // 8-bit rows out (gated)
+  static constexpr int kFeat = GATED ? kBN / 2 : kBN;                // output columns per tile
+  static constexpr int kBoxCols = kCodes ? 64 : 128 / sizeof(OutT);  // columns of a box of results
+  static constexpr int kBoxes = kFeat / 2 / kBoxCols;                // boxes of a warp
+  // boxes it has room for; a third, at the cost of a stage, brought f32 nothing
+  static constexpr int kBufs = 2;
+  static constexpr int kStages = 5;
+  static constexpr int kOffOut = kStages * kStageBytes;
+  static constexpr int kOffBar = kOffOut + 8 * kBufs * kBoxBytes;
+  // block maxima of 8-bit rows, in a second box: codes need only the first
+  static constexpr int kOffAmax = kOffOut + kBoxBytes;
+  static constexpr int kSmem = 1024 + kOffBar + 512;
+  static_assert(kSmem <= 232448, "dynamic shared memory per block");
+  static_assert(2 * 2 * kRows * 4 <= kBoxBytes, "maxima of two tiles");
+};
 
 template <bool GATED, typename OutT>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                     const __grid_constant__ CUtensorMap tmU, const __grid_constant__ CUtensorMap tmOut,
                     const __grid_constant__ CUtensorMap tmRes, const __grid_constant__ Fp8GemmParams p, bool boxes) {
-  constexpr bool kCodes = sizeof(OutT) == 1;  // 8-bit rows out (gated)
+  using PL = Plan<GATED, OutT>;
+  constexpr bool kCodes = PL::kCodes;
+  constexpr int kStages = PL::kStages, kFeat = PL::kFeat, kBoxCols = PL::kBoxCols, kBoxes = PL::kBoxes,
+                kBufs = PL::kBufs;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBar);  // [kStages] even CTA: operands of both landed
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + PL::kOffBar);  // [kStages] even CTA: operands of both landed
   uint64_t* done = full + kStages;       // [kStages] each CTA: MMA done (stage free, partial ready)
   uint64_t* acc_empty = done + kStages;  // [2] even CTA: partial read by 16 epilogue warps
-  uint64_t* res_full = acc_empty + 2;    // [8][2] each epilogue warp's boxes of the residual
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + 16);
+  uint64_t* res_full = acc_empty + 2;    // [8][kBoxes] each epilogue warp's boxes of the residual
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + 8 * kBoxes);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   uint32_t* status = p.status ? p.status : &g_fp8_status;
   // a cluster is two neighbours of the grid; said with blockIdx, the compiler
   // knows that what follows from it is the same for the whole warp
   const int rank = blockIdx.x & 1;
 
-  constexpr int kFeat = GATED ? kBN / 2 : kBN;  // output columns per tile
   const int kblocks = (p.k + kFp8Block - 1) / kFp8Block;
   const int m_tiles = (p.m + 2 * kRows - 1) / (2 * kRows), n_tiles = (p.n + kFeat - 1) / kFeat;
   const int tiles = m_tiles * n_tiles;
@@ -348,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&done[i], 1);
     }
     for (int i = 0; i < 2; ++i) mbar_init(&acc_empty[i], 16);
-    for (int i = 0; i < 16; ++i) mbar_init(&res_full[i], 1);
+    for (int i = 0; i < 8 * kBoxes; ++i) mbar_init(&res_full[i], 1);
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmW);
@@ -398,8 +412,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     regs_for_epilogue();
     const int q = warp & 3, h = (warp >> 2) - 1;  // TMEM lane quarter, column half
-    uint8_t* box = smem + kOffOut + (warp - 4) * 2 * kBoxBytes;
-    float* amax = reinterpret_cast<float*>(smem + kOffAmax);  // [tile parity][half][row of the tile]
+    uint8_t* box = smem + PL::kOffOut + (warp - 4) * kBufs * kBoxBytes;
+    float* amax = reinterpret_cast<float*>(smem + PL::kOffAmax);  // [tile parity][half][row of the tile]
     const uint32_t tlane = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * 128;
     const uint32_t empty0 = map_to_rank(&acc_empty[0], 0);
     // A tile's scales, the first block's on their way (past the last tile: the last one's).
@@ -412,20 +426,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       fetch_scales<GATED>(s, 1);
       return s;
     };
-    // Boxes of results: kBoxCols columns x this warp's 32 rows.
-    constexpr int kSize = kCodes ? 4 : static_cast<int>(sizeof(OutT));
-    constexpr int kBoxCols = 128 / kSize, kBoxes = kFeat / 2 / kBoxCols;
+    // Boxes of the residual, each with a barrier of its own that is used once a
+    // tile (so the tile's parity is the barrier's); what lies outside the matrix
+    // arrives as zeros.
     const bool res_boxes = !kCodes && !GATED && boxes && p.residual != nullptr;
-    uint64_t* res_bar = res_full + (warp - 4) * 2;
-    uint32_t res_phase = 0;  // bit b: parity of the next load into box b
-    auto fetch_residual = [&](int b, int x, int y) {  // one lane; the box is not in use
-      if (x < p.n && y < p.m) {
-        mbar_arrive_expect_tx(&res_bar[b], kBoxBytes);
-        tma_load_2d(box + b * kBoxBytes, &tmRes, &res_bar[b], x, y);
-      }
+    uint64_t* res_bar = res_full + (warp - 4) * kBoxes;
+    auto fetch_residual = [&](int c, int x, int y) {  // one lane; the box's room is not in use
+      mbar_arrive_expect_tx(&res_bar[c], kBoxBytes);
+      tma_load_2d(box + c % kBufs * kBoxBytes, &tmRes, &res_bar[c], x + c * kBoxCols, y);
     };
     Ring<kStages> ring;
-    uint32_t turn = 0;  // tiles of 8-bit rows so far
+    uint32_t turn = 0;  // tiles so far
     bool ok = true;
     Scales sc = open_tile(tile0);
     for (int tile = tile0; tile < tiles && ok; tile += tile_step) {
@@ -435,8 +446,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the residual's first boxes, once the tile before has left them
       if (res_boxes && lane == 0) {
         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        fetch_residual(0, col0, row0);
-        fetch_residual(1, col0 + kBoxCols, row0);
+#pragma unroll
+        for (int c = 0; c < kBoxes; ++c) {
+          if (c < kBufs)
+            fetch_residual(c, col0, row0);
+          else  // on its way to L2 meanwhile
+            asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(
+                             reinterpret_cast<uint64_t>(&tmRes)),
+                         "r"(col0 + c * kBoxCols), "r"(row0)
+                         : "memory");
+        }
       }
       float acc[128];
       ok = sum_blocks<GATED, 4, kStages, 2, kBN>(
@@ -460,7 +479,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < 64; j += 2) a = max_abs3_nan(a, acc[j], acc[j + 1]);
         float* shared = amax + (turn & 1) * 2 * kRows;  // the tile before may still be reading its own
-        ++turn;
         shared[h * kRows + q * 32 + lane] = a;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const float os = fp8_scale(max_nan(a, shared[(h ^ 1) * kRows + q * 32 + lane])), fac = fp8_factor(os);
@@ -490,30 +508,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         if (boxes) {
-          // Two boxes at a time: converted into shared memory (128-byte
-          // swizzle) and written by TMA stores, which clip what lies outside.
-          constexpr int kN = Pack<OutT>::kN, kPair = kBoxes < 2 ? 1 : 2;
+          // Boxes of results: converted into shared memory (128-byte swizzle)
+          // and written by TMA stores, which clip what lies outside.  Two of
+          // two boxes go together, with one fence; of four, one at a time.
+          constexpr int kN = Pack<OutT>::kN, kTogether = kBoxes == 2 ? 2 : 1;
 #pragma unroll
-          for (int c0 = 0; c0 < kBoxes; c0 += kPair) {
+          for (int c0 = 0; c0 < kBoxes; c0 += kTogether) {
             if (res_boxes) {
-              bool there = true;
 #pragma unroll
-              for (int b = 0; b < kPair; ++b)
-                if (col0 + (c0 + b) * kBoxCols < p.n && row0 < p.m) {
-                  there = there && mbar_wait(&res_bar[b], (res_phase >> b) & 1, status);
-                  res_phase ^= 1u << b;
-                }
-              ok = __all_sync(0xFFFFFFFFu, there) && ok;
+              for (int c = c0; c < c0 + kTogether; ++c)
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&res_bar[c], turn & 1, status)) && ok;
             } else {
-              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+              if (lane == 0) {
+                if (kTogether == 2)
+                  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                else
+                  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kBufs - 1) : "memory");
+              }
               __syncwarp();
             }
 #pragma unroll
-            for (int b = 0; b < kPair; ++b)
+            for (int c = c0; c < c0 + kTogether; ++c)
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
-                uint4* at = reinterpret_cast<uint4*>(box + b * kBoxBytes + lane * 128 + ((k ^ (lane & 7)) << 4));
-                float* v = acc + (c0 + b) * kBoxCols + k * kN;
+                uint4* at = reinterpret_cast<uint4*>(box + c % kBufs * kBoxBytes + lane * 128 + ((k ^ (lane & 7)) << 4));
+                float* v = acc + c * kBoxCols + k * kN;
                 if (res_boxes) Pack<OutT>::add(v, *at);
                 *at = Pack<OutT>::make(v);
               }
@@ -521,20 +540,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) {
 #pragma unroll
-              for (int b = 0; b < kPair; ++b) {
-                const int x = col0 + (c0 + b) * kBoxCols;
-                if (x < p.n && row0 < p.m)
+              for (int c = c0; c < c0 + kTogether; ++c)
+                if (col0 + c * kBoxCols < p.n && row0 < p.m)
                   asm volatile(
                       "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                           reinterpret_cast<uint64_t>(&tmOut)),
-                      "r"(smem_u32(box + b * kBoxBytes)), "r"(x), "r"(row0)
+                      "r"(smem_u32(box + c % kBufs * kBoxBytes)), "r"(col0 + c * kBoxCols), "r"(row0)
                       : "memory");
-              }
               asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-              if (kBoxes > 2 && res_boxes && c0 + 2 < kBoxes) {
-                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-#pragma unroll
-                for (int b = 0; b < 2; ++b) fetch_residual(b, col0 + (c0 + 2 + b) * kBoxCols, row0);
+              // the residual of a later box into the room of the one written before this
+              if (kBoxes > kBufs && res_boxes && c0 >= 1 && c0 - 1 + kBufs < kBoxes) {
+                asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                fetch_residual(c0 - 1 + kBufs, col0, row0);
               }
             }
           }
@@ -566,12 +583,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      ++turn;
     }
-    // Stores have to finish before the CTA ends; so do residual loads that a
-    // wait that ran out left behind.
+    // Stores have to finish before the CTA ends; so do the residual loads that
+    // a wait that ran out left behind (with a limit: some were never issued).
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     if (!ok && res_boxes)
-      for (int b = 0; b < 2; ++b) mbar_wait_limit(&res_bar[b], (res_phase >> b) & 1, status, kWaitLimitNs / 1000);
+      for (int c = 0; c < kBoxes; ++c) mbar_wait_limit(&res_bar[c], turn & 1, status, kWaitLimitNs / 1000);
   }
 
   __syncwarp();
@@ -884,7 +902,7 @@ int clusters_of(int num_sms) { return std::max(1, num_sms / 2); }
 template <bool GATED, typename OutT>
 cudaError_t launch_pair(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
   constexpr auto kernel = pair::fp8_pair_kernel<GATED, OutT>;
-  cudaError_t e = allow_smem<kernel>(pair::kSmem);
+  cudaError_t e = allow_smem<kernel>(pair::Plan<GATED, OutT>::kSmem);
   if (e != cudaSuccess) return e;
   CUtensorMap ta, tw, tu;
   if (!codes_map(&ta, p.a, p.m, p.k, p.lda, kRows) || !codes_map(&tw, p.w, p.n, p.k, p.ldw, 64) ||
@@ -907,7 +925,7 @@ cudaError_t launch_pair(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
       return cudaErrorInvalidValue;
   }
   const cudaLaunchAttribute attr = cluster_of(2);
-  return launch_pdl(kernel, dim3(2 * clusters), dim3(kThreads), pair::kSmem, st, &attr, 1, ta, tw, tu, to, tr, p,
+  return launch_pdl(kernel, dim3(2 * clusters), dim3(kThreads), pair::Plan<GATED, OutT>::kSmem, st, &attr, 1, ta, tw, tu, to, tr, p,
                     boxes);
 }
 
@@ -929,6 +947,32 @@ cudaError_t launch_tile(const Fp8GemmParams& p, int split, cudaStream_t st) {
   const cudaLaunchAttribute attr = cluster_of(split);
   return launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * split)), dim3(kThreads), kSmem, st, &attr,
                     split > 1 ? 1 : 0, ta, tw, tu, p, split, a_rows);
+}
+
+// CTAs that run at once in clusters of `split` (a power of two up to 8): a
+// cluster stays inside a group of SMs, so large ones leave some of them idle.
+template <auto KERNEL>
+int resident_ctas(int split, int smem, int num_sms) {
+  static int counts[64][4] = {};
+  int dev = 0;
+  if (split == 1 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return num_sms;
+  int& n = counts[dev][split == 2 ? 1 : split == 4 ? 2 : 3];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(num_sms / split * split));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr = cluster_of(split);
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, KERNEL, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      clusters = num_sms / split;
+    }
+    n = std::max(split, clusters * split);
+  }
+  return n;
 }
 
 struct Cost {  // us
@@ -956,9 +1000,13 @@ cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
   const bool off = sizeof(OutT) > 1 && !(p.box_o && (!p.residual || p.box_r));
   float best = c.pair_start + static_cast<float>((pairs + clusters_of(num_sms) - 1) / clusters_of(num_sms)) *
                                   (c.pair_round + c.pair_block * kblocks + (off ? 3.5f : 0.0f));
+  constexpr auto kernel = tile::fp8_tile_kernel<GATED, OutT, BN, kRows>;
+  constexpr int kSmem = tile::Plan<BN, kRows>::kSmem;
+  if (cudaError_t e = allow_smem<kernel>(kSmem); e != cudaSuccess) return e;
   int split = 0;  // pairs
   for (int s = 1; s <= 8 && s <= kblocks; s *= 2) {
-    const float rounds = static_cast<float>((tiles * s + num_sms - 1) / num_sms);
+    const int fit = resident_ctas<kernel>(s, kSmem, num_sms);
+    const float rounds = static_cast<float>((tiles * s + fit - 1) / fit);
     const float t = rounds * (c.tile + c.tile_rows * rows + c.block * static_cast<float>((kblocks + s - 1) / s) +
                               (s > 1 ? c.join : 0.0f));
     if (t < best) {
