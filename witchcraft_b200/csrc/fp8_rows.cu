@@ -3,10 +3,13 @@
 // just: scaling, the maximum and the conversion are about ten instructions an
 // element, so what a block costs beside them is shared by eight elements.
 //
-// Sixteen lanes handle one block of 128 columns, eight consecutive elements
-// each (16 bytes of 16-bit values), and a warp two blocks at a time.  VEC: every
-// row is aligned to eight elements and k is a multiple of eight, so an access
-// is either whole or absent; the other form takes the edge element by element.
+// Sixteen lanes handle one block of 128 columns, two runs of four elements
+// each, and a warp two blocks at a time.  The runs of a lane adjoin for 16-bit
+// values (16 bytes) and lie 64 columns apart for f32 (two accesses of 16 bytes
+// of which each covers whole lines: norm m = 16384, k = 768: 29.4 -> 27.1 us).
+// VEC: every row is aligned to eight elements and k is a multiple of eight, so
+// an access is either whole or absent; the other form takes the edge element by
+// element.
 #include "fp8.cuh"
 #include "fp8_rows.h"
 
@@ -18,15 +21,24 @@ constexpr int kWarps = 8;
 constexpr int kUnit = 2 * kFp8Block;  // columns a warp takes at a time
 constexpr int kHeld = 3;              // units of a row that a warp loads at once
 
+// Where a lane's runs of four lie: the first one's column within a unit, and
+// how far on the second is.
+template <bool APART>
+__device__ __forceinline__ int first_run(int lane) {
+  return APART ? (lane >> 4) * kFp8Block + (lane & 15) * 4 : lane * 8;
+}
+template <bool APART>
+constexpr int kSecond = APART ? 64 : 4;
+
 struct Eight {
   float v[8];
 };
 
 __device__ __forceinline__ float max_abs(const Eight& x) {
-  float m = fabsf(x.v[0]);
-#pragma unroll
-  for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(x.v[i]));
-  return m;
+  float m = max_abs3_nan(x.v[0], x.v[1], x.v[2]);
+  m = max_abs3_nan(m, x.v[3], x.v[4]);
+  m = max_abs3_nan(m, x.v[5], x.v[6]);
+  return max_nan(m, fabsf(x.v[7]));
 }
 __device__ __forceinline__ float half_warp_max_nan(float v) {
 #pragma unroll
@@ -39,7 +51,7 @@ __device__ __forceinline__ float warp_total(float v) {
   return v;
 }
 
-// Eight elements as they are stored.
+// Two runs of four elements as they are stored.
 template <typename T>
 struct Raw8 {
   uint4 u;
@@ -72,72 +84,79 @@ __device__ __forceinline__ Eight widen(const Raw8<__nv_bfloat16>& r) {
   }
   return e;
 }
-// Eight elements at p, of which `left` belong to the row; zeros past it.  Each
-// is read once: marked to be evicted first (norm m = 16384, k = 768: 30.2 ->
-// 28.8 us).
-template <bool VEC, typename T>
+__device__ __forceinline__ uint2 four_16bit(const uint16_t* e, int left) {
+  return make_uint2((left > 0 ? e[0] : 0u) | (left > 1 ? e[1] : 0u) << 16,
+                    (left > 2 ? e[2] : 0u) | (left > 3 ? e[3] : 0u) << 16);
+}
+// The lane's runs at p, `left` columns of the row being left from there on;
+// zeros past it.  Each is read once: marked to be evicted first (norm m = 16384,
+// k = 768: 30.2 -> 28.8 us).
+template <bool VEC, bool APART, typename T>
 __device__ __forceinline__ Raw8<T> get8(const T* p, int left) {
+  constexpr int d = kSecond<APART>;
   Raw8<T> r;
   if constexpr (sizeof(T) == 4) {
     if constexpr (VEC) {
       r.a = r.b = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (left > 0) {
-        r.a = __ldcs(reinterpret_cast<const float4*>(p));
-        r.b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-      }
+      if (left > 0) r.a = __ldcs(reinterpret_cast<const float4*>(p));
+      if (left > d) r.b = __ldcs(reinterpret_cast<const float4*>(p + d));
     } else {
       r.a = load4(p, left, false);
-      r.b = load4(p + 4, static_cast<int64_t>(left) - 4, false);
+      r.b = load4(p + d, static_cast<int64_t>(left) - d, false);
     }
-  } else if constexpr (VEC) {
-    r.u = left > 0 ? __ldcs(reinterpret_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
   } else {
-    const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (left > 2 * i ? e[2 * i] : 0u) | (left > 2 * i + 1 ? e[2 * i + 1] : 0u) << 16;
-    r.u = make_uint4(w[0], w[1], w[2], w[3]);
+    uint2 a = make_uint2(0u, 0u), b = a;
+    if constexpr (!VEC) {
+      a = four_16bit(reinterpret_cast<const uint16_t*>(p), left);
+      b = four_16bit(reinterpret_cast<const uint16_t*>(p + d), left - d);
+    } else if constexpr (APART) {
+      if (left > 0) a = __ldcs(reinterpret_cast<const uint2*>(p));
+      if (left > d) b = __ldcs(reinterpret_cast<const uint2*>(p + d));
+    } else if (left > 0) {
+      r.u = __ldcs(reinterpret_cast<const uint4*>(p));
+      return r;
+    }
+    r.u = make_uint4(a.x, a.y, b.x, b.y);
   }
   return r;
 }
-template <bool VEC, typename T>
+template <bool VEC, bool APART, typename T>
 __device__ __forceinline__ void put8(T* p, int left, const Eight& x) {
-  if constexpr (VEC) {
+  constexpr int d = kSecond<APART>;
+  if constexpr (VEC && sizeof(T) == 2 && !APART) {
     if (left <= 0) return;
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(p)[0] = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(x.v[4], x.v[5], x.v[6], x.v[7]);
-    } else {
-      T e[8];
+    T e[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x.v[i]);
-      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e);
-    }
+    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x.v[i]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e);
   } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (left > i) p[i] = from_f32<T>(x.v[i]);
+    store4(p, left, VEC, make_float4(x.v[0], x.v[1], x.v[2], x.v[3]));
+    store4(p + d, static_cast<int64_t>(left) - d, VEC, make_float4(x.v[4], x.v[5], x.v[6], x.v[7]));
   }
 }
 // The codes of eight values times f.
-template <bool VEC>
+template <bool VEC, bool APART>
 __device__ __forceinline__ void put_codes8(uint8_t* p, int left, const Eight& x, float f) {
+  constexpr int d = kSecond<APART>;
   const uint32_t a = pack_e4m3x4(x.v[0] * f, x.v[1] * f, x.v[2] * f, x.v[3] * f);
   const uint32_t b = pack_e4m3x4(x.v[4] * f, x.v[5] * f, x.v[6] * f, x.v[7] * f);
-  if (left >= 8) {
+  if (!APART && left >= 8) {
     *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
   } else if (!VEC) {
     store_codes4(p, left, a);
-    store_codes4(p + 4, static_cast<int64_t>(left) - 4, b);
+    store_codes4(p + d, static_cast<int64_t>(left) - d, b);
+  } else if (APART) {
+    if (left > 0) *reinterpret_cast<uint32_t*>(p) = a;
+    if (left > d) *reinterpret_cast<uint32_t*>(p + d) = b;
   }
 }
-// Quantises one unit of a row: eight values of this lane, of which `left`
-// belong to the row.
-template <bool VEC>
+// Quantises one unit of a row: this lane's eight values, `left` columns of the
+// row being left from its first one on.
+template <bool VEC, bool APART>
 __device__ __forceinline__ void put_unit(uint8_t* codes, float* scale, int lane, int left, const Eight& x) {
   const float s = fp8_scale(half_warp_max_nan(max_abs(x)));
   if ((lane & 15) == 0 && left > 0) *scale = s;
-  put_codes8<VEC>(codes, left, x, fp8_factor(s));
+  put_codes8<VEC, APART>(codes, left, x, fp8_factor(s));
 }
 
 // Blocks are independent: one warp per kHeld units of a row, all loads issued
@@ -150,32 +169,38 @@ __global__ void __launch_bounds__(32 * kWarps) fp8_rows_kernel(const __grid_cons
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   const int64_t row = groups == 1 ? unit : unit / groups;
   if (row >= p.m) return;
-  const int c0 = static_cast<int>(unit - row * groups) * (kHeld * kUnit) + lane * 8;
+  constexpr bool kApart = sizeof(T) == 4;
+  const int start = static_cast<int>(unit - row * groups) * (kHeld * kUnit), run = first_run<kApart>(lane);
+  const int c0 = start + run;
   const int left = static_cast<int>(p.k) - c0;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx + c0;
   uint8_t* codes = p.codes + row * p.ldc + c0;
   float* scales = p.scales + row * p.lds + c0 / kFp8Block;
   Raw8<T> v[kHeld];
 #pragma unroll
-  for (int g = 0; g < kHeld; ++g) v[g] = get8<VEC>(x + g * kUnit, left - g * kUnit);
+  for (int g = 0; g < kHeld; ++g) v[g] = get8<VEC, kApart>(x + g * kUnit, left - g * kUnit);
 #pragma unroll
   for (int g = 0; g < kHeld; ++g) {
-    if (left - g * kUnit + lane * 8 <= 0) break;  // the whole unit is past the row
-    put_unit<VEC>(codes + g * kUnit, scales + g * 2, lane, left - g * kUnit, widen(v[g]));
+    if (left - g * kUnit + run <= 0) break;  // the whole unit is past the row
+    put_unit<VEC, kApart>(codes + g * kUnit, scales + g * 2, lane, left - g * kUnit, widen(v[g]));
   }
 }
 
 // One row by WPR warps, its kHeld units per warp in registers between the sum
-// of squares and the scaling (rows up to WPR * kHeld * 256 columns).
+// of squares and the scaling (rows up to WPR * kHeld * 256 columns).  Five CTAs
+// an SM at 48 registers (norm m = 16384, k = 768: 27.1 us with four, 26.1 with
+// five, 34.3 with six, which spill): the loads of one row overlap the
+// arithmetic of the others.
 template <typename TX, typename TD, bool DELTA, bool VEC, int WPR>
-__global__ void __launch_bounds__(32 * kWarps, 3) fp8_rmsnorm_kernel(const __grid_constant__ Fp8RowsParams p) {
+__global__ void __launch_bounds__(32 * kWarps, 5) fp8_rmsnorm_kernel(const __grid_constant__ Fp8RowsParams p) {
   __shared__ float part[kWarps];
   pdl_wait();
   pdl_launch_next();
   constexpr int kStep = WPR * kUnit;  // columns between a warp's units
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wi = warp % WPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kWarps / WPR) + warp / WPR;
-  const int off = wi * kUnit + lane * 8;
+  constexpr bool kApart = sizeof(TX) == 4;
+  const int run = first_run<kApart>(lane), off = wi * kUnit + run;
   const int left0 = row < p.m ? static_cast<int>(p.k) - off : 0;  // columns from this lane's first element on
   const TX* x = static_cast<const TX*>(p.x) + row * p.ldx + off;
   const TD* d = DELTA ? static_cast<const TD*>(p.delta) + row * p.ldd + off : nullptr;
@@ -183,8 +208,8 @@ __global__ void __launch_bounds__(32 * kWarps, 3) fp8_rmsnorm_kernel(const __gri
   Raw8<TD> rd[DELTA ? kHeld : 1];
 #pragma unroll
   for (int g = 0; g < kHeld; ++g) {
-    rx[g] = get8<VEC>(x + g * kStep, left0 - g * kStep);
-    if constexpr (DELTA) rd[g] = get8<VEC>(d + g * kStep, left0 - g * kStep);
+    rx[g] = get8<VEC, kApart>(x + g * kStep, left0 - g * kStep);
+    if constexpr (DELTA) rd[g] = get8<VEC, kApart>(d + g * kStep, left0 - g * kStep);
   }
   Eight v[kHeld];
   float ss = 0.f;
@@ -215,12 +240,12 @@ __global__ void __launch_bounds__(32 * kWarps, 3) fp8_rmsnorm_kernel(const __gri
 #pragma unroll
   for (int g = 0; g < kHeld; ++g) {
     const int left = left0 - g * kStep;
-    if (left + lane * 8 <= 0) break;  // the whole unit is past the row
-    if (DELTA) put8<VEC>(sum + g * kStep, left, v[g]);
-    const Eight w = widen(get8<VEC>(p.w + off + g * kStep, left));
+    if (left + run <= 0) break;  // the whole unit is past the row
+    if (DELTA) put8<VEC, kApart>(sum + g * kStep, left, v[g]);
+    const Eight w = widen(get8<VEC, kApart>(p.w + off + g * kStep, left));
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[g].v[i] *= inv * w.v[i];
-    put_unit<VEC>(codes + g * kStep, scales + g * (kStep / kFp8Block), lane, left, v[g]);
+    put_unit<VEC, kApart>(codes + g * kStep, scales + g * (kStep / kFp8Block), lane, left, v[g]);
   }
 }
 
@@ -232,14 +257,15 @@ __global__ void __launch_bounds__(32 * kWarps) fp8_rmsnorm_wide_kernel(const __g
   pdl_launch_next();
   constexpr int kStep = kWarps * kUnit;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int off = warp * kUnit + lane * 8, k = static_cast<int>(p.k);
+  constexpr bool kApart = sizeof(TX) == 4;
+  const int off = warp * kUnit + first_run<kApart>(lane), k = static_cast<int>(p.k);
   const int64_t row = blockIdx.x;
   const TX* x = static_cast<const TX*>(p.x) + row * p.ldx + off;
   const TD* d = DELTA ? static_cast<const TD*>(p.delta) + row * p.ldd + off : nullptr;
   auto value = [&](int c) {
-    Eight v = widen(get8<VEC>(x + c, k - off - c));
+    Eight v = widen(get8<VEC, kApart>(x + c, k - off - c));
     if constexpr (DELTA) {
-      const Eight e = widen(get8<VEC>(d + c, k - off - c));
+      const Eight e = widen(get8<VEC, kApart>(d + c, k - off - c));
 #pragma unroll
       for (int i = 0; i < 8; ++i) v.v[i] += e.v[i];
     }
@@ -264,11 +290,11 @@ __global__ void __launch_bounds__(32 * kWarps) fp8_rmsnorm_wide_kernel(const __g
   for (int c = 0; c < k - warp * kUnit; c += kStep) {
     const int left = k - off - c;
     Eight v = value(c);
-    if (DELTA) put8<VEC>(sum + c, left, v);
-    const Eight w = widen(get8<VEC>(p.w + off + c, left));
+    if (DELTA) put8<VEC, kApart>(sum + c, left, v);
+    const Eight w = widen(get8<VEC, kApart>(p.w + off + c, left));
 #pragma unroll
     for (int i = 0; i < 8; ++i) v.v[i] *= inv * w.v[i];
-    put_unit<VEC>(p.codes + row * p.ldc + off + c, p.scales + row * p.lds + (off + c) / kFp8Block, lane, left, v);
+    put_unit<VEC, kApart>(p.codes + row * p.ldc + off + c, p.scales + row * p.lds + (off + c) / kFp8Block, lane, left, v);
   }
 }
 
@@ -278,16 +304,17 @@ __global__ void __launch_bounds__(32 * kWarps) fp8_weight_kernel(const __grid_co
   __shared__ float part[kWarps];
   pdl_wait();
   pdl_launch_next();
+  constexpr bool kApart = sizeof(T) == 4;
   constexpr int kTurns = kFp8Block / (2 * kWarps);  // a warp takes two rows at a time
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t nb = blockIdx.x / kblocks, kb = blockIdx.x % kblocks;
-  const int64_t row0 = nb * kFp8Block + warp * 2 + (lane >> 4), col = kb * kFp8Block + (lane & 15) * 8;
+  const int64_t row0 = nb * kFp8Block + warp * 2 + (lane >> 4), col = kb * kFp8Block + first_run<kApart>(lane & 15);
   const int left = static_cast<int>(p.k - col);
   const T* x = static_cast<const T*>(p.x) + row0 * p.ldx + col;
   Raw8<T> v[kTurns];
 #pragma unroll
   for (int t = 0; t < kTurns; ++t)
-    v[t] = get8<VEC>(x + 2 * kWarps * t * p.ldx, row0 + 2 * kWarps * t < p.m ? left : 0);
+    v[t] = get8<VEC, kApart>(x + 2 * kWarps * t * p.ldx, row0 + 2 * kWarps * t < p.m ? left : 0);
   float a = 0.f;
 #pragma unroll
   for (int t = 0; t < kTurns; ++t) a = max_nan(a, max_abs(widen(v[t])));
@@ -301,7 +328,7 @@ __global__ void __launch_bounds__(32 * kWarps) fp8_weight_kernel(const __grid_co
 #pragma unroll
   for (int t = 0; t < kTurns; ++t) {
     const int64_t row = row0 + 2 * kWarps * t;
-    if (row < p.m) put_codes8<VEC>(p.codes + row * p.ldc + col, left, widen(v[t]), f);
+    if (row < p.m) put_codes8<VEC, kApart>(p.codes + row * p.ldc + col, left, widen(v[t]), f);
   }
 }
 
