@@ -906,8 +906,9 @@ cudaError_t launch_pair(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   CUtensorMap ta, tw, tu;
   if (!codes_map(&ta, p.a, p.m, p.k, p.lda, kRows) || !codes_map(&tw, p.w, p.n, p.k, p.ldw, 64) ||
-      !codes_map(&tu, GATED ? p.up : p.w, p.n, p.k, GATED ? p.ldup : p.ldw, 64))
+      (GATED && !codes_map(&tu, p.up, p.n, p.k, p.ldup, 64)))
     return cudaErrorInvalidValue;
+  if (!GATED) tu = tw;
   constexpr int kFeat = GATED ? pair::kBN / 2 : pair::kBN;
   const int64_t tiles = static_cast<int64_t>((p.m + 2 * kRows - 1) / (2 * kRows)) * ((p.n + kFeat - 1) / kFeat);
   if (tiles > 0x40000000 || tiles * ((p.k + kFp8Block - 1) / kFp8Block) > 0xFFFFFFFFll * clusters_of(num_sms))
@@ -939,8 +940,9 @@ cudaError_t launch_tile(const Fp8GemmParams& p, int split, cudaStream_t st) {
   const int a_rows = std::min(A_ROWS, (p.m + 7) / 8 * 8);
   CUtensorMap ta, tw, tu;
   if (!codes_map(&ta, p.a, p.m, p.k, p.lda, a_rows) || !codes_map(&tw, p.w, p.n, p.k, p.ldw, 64) ||
-      !codes_map(&tu, GATED ? p.up : p.w, p.n, p.k, GATED ? p.ldup : p.ldw, 64))
+      (GATED && !codes_map(&tu, p.up, p.n, p.k, p.ldup, 64)))
     return cudaErrorInvalidValue;
+  if (!GATED) tu = tw;
   constexpr int kFeat = GATED ? BN / 2 : BN;
   const int64_t tiles = static_cast<int64_t>((p.m + kRows - 1) / kRows) * ((p.n + kFeat - 1) / kFeat);
   if (tiles * split > 0x7FFFFFFF) return cudaErrorInvalidValue;

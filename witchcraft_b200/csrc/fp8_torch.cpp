@@ -4,6 +4,8 @@
 // functions come in as addresses of the library that witchcraft_b200._lib
 // loaded, so there is one instance of it.
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -80,14 +82,18 @@ int64_t codes_ld(const Tensor& t) {
   return t.size(0) > 1 ? t.stride(0) : (std::max(t.stride(0), t.size(1)) + 15) / 16 * 16;
 }
 
-Tensor empty(int64_t r, int64_t c, at::ScalarType type, c10::Device device) {
-  return at::empty({r, c}, at::TensorOptions().dtype(type).device(device));
+// An uninitialised tensor on the current device (the callers' guards make it
+// the operands'): torch's CUDA allocator without its dispatcher.
+Tensor empty_bytes(c10::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_generic(sizes, c10::cuda::CUDACachingAllocator::get(),
+                                   c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
 }
+Tensor empty(int64_t r, int64_t c, at::ScalarType type) { return empty_bytes({r, c}, type); }
 // Codes [r][c] and scales [sr][ceil(c / 128)] in one allocation (an allocation
 // costs about as much as a launch): two tensors over one storage.
-std::tuple<Tensor, Tensor> empty_quantized(int64_t r, int64_t c, int64_t sr, c10::Device device) {
+std::tuple<Tensor, Tensor> empty_quantized(int64_t r, int64_t c, int64_t sr) {
   const int64_t wide = (c + 15) / 16 * 16, kb = blocks(c), offset = (r * wide + 255) / 256 * 64;  // in floats
-  const Tensor buf = at::empty({4 * (offset + sr * kb)}, at::TensorOptions().dtype(at::kByte).device(device));
+  const Tensor buf = empty_bytes({4 * (offset + sr * kb)}, at::kByte);
   auto over = [&](at::ScalarType type, int64_t at0, int64_t rows, int64_t cols, int64_t ld) {
     Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(),
                                                         c10::scalarTypeToTypeMeta(type));
@@ -118,7 +124,7 @@ Pair quantize(const Tensor& x) {
   columns(x, "x");
   const int64_t m = x.size(0), k = x.size(1);
   const c10::cuda::CUDAGuard guard(x.device());
-  auto [codes, scales] = empty_quantized(m, k, m, x.device());
+  auto [codes, scales] = empty_quantized(m, k, m);
   if (m)
     check(api.rows(x.data_ptr(), code, m, k, ld(x), codes.data_ptr(), codes_ld(codes), floats(scales), scales.size(1),
                    stream_of(x)));
@@ -130,7 +136,7 @@ Pair quantize_weight(const Tensor& w) {
   const int64_t n = w.size(0), k = w.size(1);
   if (n < 1 || k < 1) refuse("w is empty");
   const c10::cuda::CUDAGuard guard(w.device());
-  auto [codes, scales] = empty_quantized(n, k, blocks(n), w.device());
+  auto [codes, scales] = empty_quantized(n, k, blocks(n));
   check(api.weight(w.data_ptr(), code, n, k, ld(w), codes.data_ptr(), codes_ld(codes), floats(scales), scales.size(1),
                    stream_of(w)));
   return {codes, scales};
@@ -156,8 +162,8 @@ py::tuple rmsnorm(const Tensor& x, const Tensor& weight, double eps, const std::
     }
   }
   const c10::cuda::CUDAGuard guard(x.device());
-  Tensor sum = !delta ? Tensor() : out ? *out : empty(m, k, x.scalar_type(), x.device());
-  auto [codes, scales] = empty_quantized(m, k, m, x.device());
+  Tensor sum = !delta ? Tensor() : out ? *out : empty(m, k, x.scalar_type());
+  auto [codes, scales] = empty_quantized(m, k, m);
   if (m)
     check(api.rmsnorm(x.data_ptr(), code, ld(x), delta ? delta->data_ptr() : nullptr, dcode, delta ? ld(*delta) : 0,
                       delta ? sum.data_ptr() : nullptr, delta ? ld(sum) : 0, floats(weight), m, k,
@@ -190,7 +196,7 @@ Tensor matmul(const Tensor& a, const Tensor& a_scales, const Tensor& w, const Te
     sized(*out, "out", m, n);
     y = *out;
   } else {
-    y = empty(m, n, type, a.device());
+    y = empty(m, n, type);
   }
   if (m)
     check(api.matmul(a.data_ptr(), codes_ld(a), floats(a_scales), ld(a_scales), m, k, w.data_ptr(), codes_ld(w),
@@ -216,9 +222,9 @@ py::object gated_matmul(const Tensor& a, const Tensor& a_scales, const Tensor& g
   const c10::cuda::CUDAGuard guard(a.device());
   Tensor y, scales;
   if (out_dtype)
-    y = empty(m, n, *out_dtype, a.device());
+    y = empty(m, n, *out_dtype);
   else
-    std::tie(y, scales) = empty_quantized(m, n, m, a.device());
+    std::tie(y, scales) = empty_quantized(m, n, m);
   if (m)
     check(api.gated(a.data_ptr(), codes_ld(a), floats(a_scales), ld(a_scales), m, k, gate.data_ptr(), codes_ld(gate),
                     floats(gate_scales), ld(gate_scales), up.data_ptr(), codes_ld(up), floats(up_scales),
