@@ -424,3 +424,34 @@ def test_refusals_on_the_gpu():
         fp8.matmul(torch.empty(4, 260, dtype=torch.float8_e4m3fn, device="cuda")[:, :256], sa, w, sw)
     with pytest.raises(fp8.WcError, match="16 bytes"):
         fp8.matmul(fp8.empty_codes(4, 512, "cuda")[:, 8:264], sa, w, sw)
+
+
+# ---------------------------------------------------------------- the operators together
+
+@pytest.mark.parametrize("tokens", [1, 32, 700])
+def test_feed_forward_example(tiny_model, tokens):
+    """The example's block (norm, gate, product) against the same block in f32.
+
+    Every code is off by at most 2^-4 of its value (3 fraction bits), about
+    evenly spread: 2^-4 / sqrt(3) = 0.036 in the mean square at worst.  The first product has two
+    such factors (0.051); the gate multiplies two results of it (slope of GELU
+    at most 1.13: 0.077), its rows are rounded again (0.085 with 0.036), and the
+    last weights too (0.093).  Twice that bounds what the block adds."""
+    import importlib.util
+    import os
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("fp8_feed_forward",
+                                                  os.path.join(ROOT, "examples", "fp8_feed_forward.py"))
+    example = importlib.util.module_from_spec(spec)
+    import sys
+    sys.modules[spec.name] = example
+    spec.loader.exec_module(example)
+    block = example.FeedForward.load(tiny_model, 1)
+    d = tiny_model.config.d_model
+    x, attention = randn(tokens, d, seed=tokens), randn(tokens, d, seed=2, dtype=torch.float16)
+    keep = x.clone()
+    y, want = block(x, attention), example.reference(tiny_model, 1, x, attention)
+    assert torch.equal(x, keep)
+    added = want - x - attention.float()
+    assert float((y - want).norm() / added.norm()) < 0.19
+    fp8.synchronize()

@@ -439,7 +439,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t turn = 0;  // tiles so far
     bool ok = true;
     Scales sc = open_tile(tile0);
-    for (int tile = tile0; tile < tiles && ok; tile += tile_step) {
+    // 8-bit rows meet at a barrier once a tile: a warp whose wait ran out goes on
+    // meeting the others there
+    for (int tile = tile0; tile < tiles && (ok || kCodes); tile += tile_step) {
       const int m0 = (tile / n_tiles) * 2 * kRows + rank * kRows;
       const int f0 = (tile % n_tiles) * kFeat;
       const int row0 = m0 + q * 32, col0 = f0 + h * (kFeat / 2);  // this warp's first row and output column
@@ -458,12 +460,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       float acc[128];
-      ok = sum_blocks<GATED, 4, kStages, 2, kBN>(
+      ok = ok && sum_blocks<GATED, 4, kStages, 2, kBN>(
           acc, sc, kblocks, 1, tlane, done, ring, status,
           [&](uint32_t buf) {
             if (lane == 0) mbar_arrive_remote(empty0 + buf * 8);
           });
-      if (!ok) break;
+      if (!ok && !kCodes) break;
       sc = open_tile(tile + tile_step);  // arrives while this tile is written
 
       const int row = row0 + lane;
@@ -474,7 +476,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if constexpr (kCodes) {
         // The 64 results of this thread and those of the thread with the same
-        // row in the other half are one block of 128.
+        // row in the other half are one block of 128 (without what lies past the
+        // last feature: 0, or NaN where a scale is infinite).
+        if (col0 + 64 > p.n) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) acc[j] = col0 + j < p.n ? acc[j] : 0.f;
+        }
         float a = 0.f;
 #pragma unroll
         for (int j = 0; j < 64; j += 2) a = max_abs3_nan(a, acc[j], acc[j + 1]);
@@ -780,8 +787,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int c = (lane >> 4) * 32 + (lane & 15);
         const float4 g = total(r, c), u = total(r, c + 16);
         const Gate gate(p.act);
-        const float4 v = make_float4(gate(g.x, u.x), gate(g.y, u.y), gate(g.z, u.z), gate(g.w, u.w));
-        const int col = f0 + lane * 4;
+        const int col = f0 + lane * 4, left = p.n - col;  // past the last feature: 0, whatever the scales are
+        const float4 v = make_float4(left > 0 ? gate(g.x, u.x) : 0.f, left > 1 ? gate(g.y, u.y) : 0.f,
+                                     left > 2 ? gate(g.z, u.z) : 0.f, left > 3 ? gate(g.w, u.w) : 0.f);
         if constexpr (kCodes) {
           const float a = max_abs3_nan(max_abs3_nan(v.x, v.y, v.z), v.w, v.w);
           const float sc = fp8_scale(warp_max_nan(a)), fac = fp8_factor(sc);
