@@ -317,9 +317,10 @@ struct Plan {
   static constexpr int kFeat = GATED ? kBN / 2 : kBN;                // output columns per tile
   static constexpr int kBoxCols = kCodes ? 64 : 128 / sizeof(OutT);  // columns of a box of results
   static constexpr int kBoxes = kFeat / 2 / kBoxCols;                // boxes of a warp
-  // boxes it has room for; a third, at the cost of a stage, brought f32 nothing
-  static constexpr int kBufs = 2;
-  static constexpr int kStages = 5;
+  // boxes it has room for: a third for f32, at the cost of a stage (16384 x 768
+  // x 768 with residual: 30.0 -> 27.1 us, 16384 x 2048 x 768: 42.5 -> 40.9)
+  static constexpr int kBufs = kBoxes > 2 ? 3 : 2;
+  static constexpr int kStages = kBufs == 3 ? 4 : 5;
   static constexpr int kOffOut = kStages * kStageBytes;
   static constexpr int kOffBar = kOffOut + 8 * kBufs * kBoxBytes;
   // block maxima of 8-bit rows, in a second box: codes need only the first
@@ -542,6 +543,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float* v = acc + c * kBoxCols + k * kN;
                 if (res_boxes) Pack<OutT>::add(v, *at);
                 *at = Pack<OutT>::make(v);
+                // not the whole box of the residual in registers at once: it would spill
+                if (sizeof(OutT) == 4 && (k & 1)) asm volatile("" ::: "memory");
               }
             fence_proxy_async_smem();
             __syncwarp();
