@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from witchcraft_b200 import fp8
+from witchcraft_b200._lib import lib
 
 pytestmark = pytest.mark.gpu
 
@@ -338,6 +339,67 @@ def test_strided_and_unaligned_operands(m):
     c, s = fp8.gated_matmul(a, sa, w, sw, w, sw)
     c0, s0 = fp8.gated_matmul(a0, sa0, w0, sw0, w0, sw0)
     assert torch.equal(c.float(), c0.float()) and torch.equal(s, s0)
+
+
+@pytest.mark.parametrize("n,start,res_start", [(701, 1, 6), (512, 3, 0), (513, 0, 5), (130, 7, 2), (6, 2, 3), (1, 5, 7)])
+@pytest.mark.parametrize("dtype", TYPES.values(), ids=TYPES)
+def test_many_rows_off_the_boundary(n, start, res_start, dtype):
+    """Rows of results and of the residual that start anywhere in a 16-byte
+    block, each at its own place; what surrounds them stays as it is."""
+    m, k = 8003, 140
+    a, sa, (gate, up) = operands(m, k, n, seed=n, mats=2)
+    frame = torch.full((m + 1, n + 11), 7.0, dtype=dtype, device="cuda")
+    out = frame[1:, start:start + n]
+    res = randn(m, n + 9, seed=start, dtype=dtype)[:, res_start:res_start + n]
+
+    def near(y, want, err):
+        return ((y.double() - want).abs() <= err + ROUND[dtype] * (want.abs() + err) + 2.0 ** -25).all()
+
+    def check(want, err):
+        assert near(out, want, err)
+        out.fill_(7.0)
+        assert (frame == 7.0).all()
+
+    y, err = product64(a, sa, *gate)
+    fp8.matmul(a, sa, *gate, dtype, out=out)
+    check(y, err)
+    fp8.matmul(a, sa, *gate, dtype, residual=res, out=out)
+    y = y + res.double()
+    check(y, err + U * y.abs())
+    out.copy_(res)
+    fp8.matmul(a, sa, *gate, dtype, residual=out, out=out)
+    check(y, err + U * y.abs())
+    assert near(fp8.gated_matmul(a, sa, *gate, *up, out_dtype=dtype), *gated64(a, sa, gate, up, "gelu"))
+
+
+@pytest.mark.parametrize("m", [3, 130, 5000])
+@pytest.mark.parametrize("n", [64, 100, 129, 250, 328])
+def test_codes_end_where_the_row_ends(m, n):
+    """8-bit rows into wider ones: the bytes behind them stay as they are."""
+    k, ld = 300, 384
+    a, sa, (gate, up) = operands(m, k, n, seed=n, mats=2)
+    x, w = randn(m, n, seed=1), torch.ones(n, device="cuda")
+    frame = torch.empty(m, ld, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(m, 5, device="cuda")
+    blocks = -(-n // 128)
+
+    def check(call, codes, s):
+        frame.fill_(0x55)
+        scales.fill_(7.0)
+        assert call(frame.data_ptr(), ld, scales.data_ptr(), 5) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(frame[:, :n], codes.view(torch.uint8)) and (frame[:, n:] == 0x55).all()
+        assert torch.equal(scales[:, :blocks], s) and (scales[:, blocks:] == 7.0).all()
+
+    f32, e4m3, stream = 0, 3, torch.cuda.current_stream().cuda_stream
+    mat = lambda t: (t.data_ptr(), t.stride(0))
+    check(lambda c, ldc, s, lds: lib().wc_fp8_quantize_rows(x.data_ptr(), f32, m, n, n, c, ldc, s, lds, stream),
+          *fp8.quantize(x))
+    check(lambda c, ldc, s, lds: lib().wc_fp8_rmsnorm(x.data_ptr(), f32, n, None, f32, 0, None, 0, w.data_ptr(), m, n, 1e-6,
+                                                      c, ldc, s, lds, stream), *fp8.rmsnorm(x, w))
+    check(lambda c, ldc, s, lds: lib().wc_fp8_gated_matmul(
+        *mat(a), *mat(sa), m, k, *mat(gate[0]), *mat(gate[1]), *mat(up[0]), *mat(up[1]), n, 0, c, e4m3, ldc, s, lds, stream),
+        *fp8.gated_matmul(a, sa, *gate, *up))
 
 
 def test_product_offsets_past_32_bits():

@@ -33,8 +33,13 @@ bool aligned(const void* p, int64_t ld, int bytes, int type) {  // rows start at
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (ld * type_size(type)) % bytes == 0;
 }
 // rows of eight elements at a time: 16-byte accesses
+// Whether rows of n results can be written by TMA boxes, which end a row at a
+// multiple of 16 bytes: a row that ends between two would take the bytes behind
+// it along (zeros there).
+bool boxes(const void* p, int64_t ld, int64_t n, int type) {
+  return aligned(p, ld, 16, type) && n * type_size(type) % 16 == 0;
+}
 bool vec8(const void* p, int64_t ld, int type) { return aligned(p, ld, 16, type) && ld % 8 == 0; }
-bool vec4(const void* p, int64_t ld, int type) { return aligned(p, ld, 4 * type_size(type), type); }
 bool natural(const void* p, int type) { return reinterpret_cast<uintptr_t>(p) % type_size(type) == 0; }
 int64_t blocks(int64_t k) { return (k + 127) / 128; }
 
@@ -193,9 +198,7 @@ extern "C" int wc_fp8_matmul(const void* d_a, int64_t lda, const float* d_sa, in
   p.out = d_out;
   p.ldr = ldr;
   p.ldo = ldo;
-  p.vec_o = vec4(d_out, ldo, out_type);
-  p.vec_r = d_residual && vec4(d_residual, ldr, out_type);
-  p.box_o = aligned(d_out, ldo, 16, out_type);
+  p.box_o = boxes(d_out, ldo, n, out_type);
   p.box_r = d_residual && aligned(d_residual, ldr, 16, out_type);
   return done(fp8_gemm_launch(false, out_type, p, sms, static_cast<cudaStream_t>(stream)), "product launch");
 }
@@ -228,8 +231,7 @@ extern "C" int wc_fp8_gated_matmul(const void* d_a, int64_t lda, const float* d_
   p.ldo = ldo;
   p.out_scales = d_out_scales;
   p.ldos = ldos;
-  p.vec_o = vec4(d_out, ldo, out_type);
-  p.box_o = aligned(d_out, ldo, 16, out_type);
+  p.box_o = boxes(d_out, ldo, n, out_type);
   return done(fp8_gemm_launch(true, out_type, p, sms, static_cast<cudaStream_t>(stream)), "gated product launch");
 }
 

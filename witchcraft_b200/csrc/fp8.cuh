@@ -1,6 +1,8 @@
 // Shared by the 8-bit operators (fp8_rows.cu, fp8_gemm.cu): element types,
 // the e4m3 conversion and the scale of a block.
 #pragma once
+
+#include <type_traits>
 #include "common.cuh"
 
 #include "../../include/wc_fp8.h"
@@ -67,34 +69,48 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Four consecutive elements at p (of a row with `left` elements from p on) as
-// f32, zeros past the row's end.  vec: p is aligned to four elements.
+// Four consecutive elements at p (of a row with `left` elements from p on),
+// zeros past the row's end, first as loaded and then as f32, so that many loads
+// are on their way before the first is used.  Rows may start at any element.
 template <typename T>
-__device__ __forceinline__ float4 load4(const T* p, int64_t left, bool vec) {
-  if (vec && left >= 4) {
-    if constexpr (sizeof(T) == 4) {
-      return *reinterpret_cast<const float4*>(p);
+struct Raw4 {
+  uint32_t w[4];  // 16-bit: four elements in two words, or one in each
+  bool whole = false;
+  __device__ __forceinline__ void load(const T* p, int64_t left) {
+    whole = left >= 4 && reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0;
+    if (whole) {
+      if constexpr (sizeof(T) == 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[0] = u.x, w[1] = u.y;
+      }
     } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+      const Bits* e = reinterpret_cast<const Bits*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = left > i ? e[i] : 0u;
+    }
+  }
+  __device__ __forceinline__ float4 value() const {
+    if constexpr (sizeof(T) == 4) {
+      return make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]), __uint_as_float(w[3]));
+    } else {
+      const uint2 u = whole ? make_uint2(w[0], w[1]) : make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
       const T* e = reinterpret_cast<const T*>(&u);
       return make_float4(to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3]));
     }
   }
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (left > 0) v.x = to_f32(p[0]);
-  if (left > 1) v.y = to_f32(p[1]);
-  if (left > 2) v.z = to_f32(p[2]);
-  if (left > 3) v.w = to_f32(p[3]);
-  return v;
-}
+};
 template <typename T>
-__device__ __forceinline__ void store4(T* p, int64_t left, bool vec, float4 v) {
-  if (vec && left >= 4) {
+__device__ __forceinline__ void store4(T* p, int left, float4 v) {
+  if (left >= 4 && reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0) {
     if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<float4*>(p) = v;
     } else {
-      T e[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
-      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(e);
+      const T e[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
     }
     return;
   }
@@ -112,12 +128,5 @@ __device__ __forceinline__ void store_codes4(uint8_t* p, int64_t left, uint32_t 
   for (int i = 0; i < 3; ++i)
     if (left > i) p[i] = static_cast<uint8_t>(c >> (8 * i));
 }
-
-// Host side: whether rows of `ld` elements from p are aligned to four
-// elements of `size` bytes.
-inline bool aligned4(const void* p, int64_t ld, int size) {
-  return (reinterpret_cast<uintptr_t>(p) % (4 * size)) == 0 && ld % 4 == 0;
-}
-inline int fp8_type_size(int t) { return t == WC_T_F32 ? 4 : t == WC_T_E4M3 ? 1 : 2; }
 
 }  // namespace wc

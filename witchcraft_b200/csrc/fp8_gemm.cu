@@ -308,10 +308,11 @@ namespace pair {
 constexpr int kBN = 256;
 constexpr int kStageBytes = kABytes + 128 * kFp8Block;
 constexpr int kBoxBytes = 32 * 128;  // 32 rows x 128 bytes of results (or of the residual)
+constexpr int kPitch = 128 + 16;     // of such a row that starts inside a block of 16 bytes
 
 // Shared memory: operand stages, then boxes of results for each epilogue warp
 // (a warp's results are four boxes of f32 or two of 16-bit values).
-template <bool GATED, typename OutT>
+template <bool GATED, typename OutT, bool BOXES>
 struct Plan {
   static constexpr bool kCodes = sizeof(OutT) == 1;  // 8-bit rows out (gated)
   static constexpr int kFeat = GATED ? kBN / 2 : kBN;                // output columns per tile
@@ -319,23 +320,45 @@ struct Plan {
   static constexpr int kBoxes = kFeat / 2 / kBoxCols;                // boxes of a warp
   // boxes it has room for: a third for f32, at the cost of a stage (16384 x 768
   // x 768 with residual: 30.0 -> 27.1 us, 16384 x 2048 x 768: 42.5 -> 40.9)
-  static constexpr int kBufs = kBoxes > 2 ? 3 : 2;
+  static constexpr int kBufs = kBoxes > 2 || !BOXES ? 3 : 2;
   static constexpr int kStages = kBufs == 3 ? 4 : 5;
   static constexpr int kOffOut = kStages * kStageBytes;
   static constexpr int kOffBar = kOffOut + 8 * kBufs * kBoxBytes;
   // block maxima of 8-bit rows, in a second box: codes need only the first
   static constexpr int kOffAmax = kOffOut + kBoxBytes;
   static constexpr int kSmem = 1024 + kOffBar + 512;
+  static_assert(BOXES || 2 * 32 * kPitch <= kBufs * kBoxBytes, "two turns of rows off the 16-byte boundary");
   static_assert(kSmem <= 232448, "dynamic shared memory per block");
   static_assert(2 * 2 * kRows * 4 <= kBoxBytes, "maxima of two tiles");
 };
 
-template <bool GATED, typename OutT>
+__device__ __forceinline__ uint32_t load_shared(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 load_shared4(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_shared(uint32_t at, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ void store_shared(uint32_t at, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// BOXES: results (and the residual) move by TMA boxes, which wants rows that
+// start at multiples of 16 bytes.  The way out for other rows would cost the
+// kernel registers even where it is not taken (f32 results 45.8 -> 50.9 us at
+// 16384 x 768 x 2304).
+template <bool GATED, typename OutT, bool BOXES>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                     const __grid_constant__ CUtensorMap tmU, const __grid_constant__ CUtensorMap tmOut,
-                    const __grid_constant__ CUtensorMap tmRes, const __grid_constant__ Fp8GemmParams p, bool boxes) {
-  using PL = Plan<GATED, OutT>;
+                    const __grid_constant__ CUtensorMap tmRes, const __grid_constant__ Fp8GemmParams p) {
+  using PL = Plan<GATED, OutT, BOXES>;
   constexpr bool kCodes = PL::kCodes;
   constexpr int kStages = PL::kStages, kFeat = PL::kFeat, kBoxCols = PL::kBoxCols, kBoxes = PL::kBoxes,
                 kBufs = PL::kBufs;
@@ -430,7 +453,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Boxes of the residual, each with a barrier of its own that is used once a
     // tile (so the tile's parity is the barrier's); what lies outside the matrix
     // arrives as zeros.
-    const bool res_boxes = !kCodes && !GATED && boxes && p.residual != nullptr;
+    const bool res_boxes = !kCodes && !GATED && BOXES && p.residual != nullptr;
+    const bool res_rows = !kCodes && !GATED && !BOXES && p.residual != nullptr;
     uint64_t* res_bar = res_full + (warp - 4) * kBoxes;
     auto fetch_residual = [&](int c, int x, int y) {  // one lane; the box's room is not in use
       mbar_arrive_expect_tx(&res_bar[c], kBoxBytes);
@@ -459,6 +483,36 @@ __global__ void __launch_bounds__(kThreads, 1)
                          "r"(col0 + c * kBoxCols), "r"(row0)
                          : "memory");
         }
+      }
+      // the same for rows off the 16-byte boundary: the 16-byte blocks that hold
+      // 128 bytes of a row from its start's block on, a bulk copy per row (what a
+      // block holds of other rows is not used)
+      const int res_bytes = row0 + lane < p.m ? max(0, min(p.n - col0, kFeat / 2)) * static_cast<int>(sizeof(OutT)) : 0;
+      auto residual_row = [&] {
+        return static_cast<const OutT*>(p.residual) + static_cast<int64_t>(row0 + lane) * p.ldr + col0;
+      };
+      auto fetch_rows = [&](int t) {
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(residual_row());
+        const int start = static_cast<int>(reinterpret_cast<uintptr_t>(from) & 15);
+        const int end = res_bytes ? (start + res_bytes + 15) & ~15 : 0;
+        const int size = max(0, min(end - t * 128, kPitch));
+        const uint32_t sum = __reduce_add_sync(0xFFFFFFFFu, static_cast<uint32_t>(size));
+        if (lane == 0) mbar_arrive_expect_tx(&res_bar[t], sum);
+        __syncwarp();
+        if (size > 0)
+          asm volatile(
+              "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                  smem_u32(box + (t % 2 * 32 + lane) * kPitch)),
+              "l"(from - start + t * 128), "r"(size), "r"(smem_u32(&res_bar[t]))
+              : "memory");
+      };
+      if (res_rows) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        fetch_rows(0);
+        if (kBoxes > 1) fetch_rows(1);
+        for (int c = 256; c < res_bytes; c += 128)  // on its way to L2 meanwhile
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint8_t*>(residual_row()) + c));
       }
       float acc[128];
       ok = ok && sum_blocks<GATED, 4, kStages, 2, kBN>(
@@ -491,9 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const float os = fp8_scale(max_nan(a, shared[(h ^ 1) * kRows + q * 32 + lane])), fac = fp8_factor(os);
         if (h == 0 && row < p.m) p.out_scales[row * p.ldos + f0 / kFp8Block] = os;
-        // 32 rows x 64 codes by one TMA store (64-byte swizzle)
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        __syncwarp();
+        uint4 code[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {  // 16 codes
           uint32_t w[4];
@@ -501,21 +553,46 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 4; ++e)
             w[e] = pack_e4m3x4(acc[16 * c + 4 * e] * fac, acc[16 * c + 4 * e + 1] * fac, acc[16 * c + 4 * e + 2] * fac,
                                acc[16 * c + 4 * e + 3] * fac);
-          *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          code[c] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          if (col0 < p.n && row0 < p.m)
-            asm volatile(
-                "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
-                    reinterpret_cast<uint64_t>(&tmOut)),
-                "r"(smem_u32(box)), "r"(col0), "r"(row0)
-                : "memory");
-          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        if (col0 + 64 > p.n && p.n % 16 != 0) {
+          // The rows end here inside 16 bytes, which a TMA store would write to
+          // their end: each lane writes its own.
+          if (row < p.m) {
+            uint8_t* to = static_cast<uint8_t*>(p.out) + static_cast<int64_t>(row) * p.ldo + col0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int left = p.n - col0 - 16 * c;
+              const uint32_t w[4] = {code[c].x, code[c].y, code[c].z, code[c].w};
+              if (left >= 16) {
+                *reinterpret_cast<uint4*>(to + 16 * c) = code[c];
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) store_codes4(to + 16 * c + 4 * e, left - 4 * e, w[e]);
+              }
+            }
+          }
+        } else {
+          // 32 rows x 64 codes by one TMA store (64-byte swizzle)
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = code[c];
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (col0 < p.n && row0 < p.m)
+              asm volatile(
+                  "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                      reinterpret_cast<uint64_t>(&tmOut)),
+                  "r"(smem_u32(box)), "r"(col0), "r"(row0)
+                  : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
         }
       } else {
-        if (boxes) {
+        if constexpr (BOXES) {
           // Boxes of results: converted into shared memory (128-byte swizzle)
           // and written by TMA stores, which clip what lies outside.  Two of
           // two boxes go together, with one fence; of four, one at a time.
@@ -566,29 +643,108 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         } else {
-          // Rows off the 16-byte boundary: 32 columns at a time through shared
-          // memory, then element by element, a lane per column.
+          // Rows off the 16-byte boundary.  A lane lays its row out in shared
+          // memory as it will lie in global memory, counted from the 16-byte
+          // block in which the row starts (so a 16-bit row may begin inside a
+          // word), 128 bytes at a time; then eight lanes write a row, whole
+          // blocks as such, the blocks that it owns in part by elements.  The
+          // words of a block are turned by one for every eight rows, which
+          // would else share their banks.  16384 x 768 x 2302, f16: 46.2 us, with
+          // residual 71.8 (2304 columns in boxes: 36.2 and 46.4); element by
+          // element it was 77 and 301, by a bulk copy per row 72 and 102.
+          constexpr int kSize = sizeof(OutT), kPer = 4 / kSize;
           OutT* out = static_cast<OutT*>(p.out);
-          const OutT* res = static_cast<const OutT*>(p.residual);
-          float* f = reinterpret_cast<float*>(box);
-          const int left = min(32, p.m - row0);
+          const int bytes = max(0, min(p.n - col0, kFeat / 2)) * kSize;  // of a row
+          auto start_of = [](const OutT* at) { return static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15); };
+          const int own_start = start_of(out + static_cast<int64_t>(row0 + lane) * p.ldo + col0);
+          const uint32_t rows_of_warp = smem_u32(box);
+          uint32_t word[4];  // where words 0 to 3 of the row go
 #pragma unroll
-          for (int c = 0; c < kFeat / 64; ++c) {
-            __syncwarp();
+          for (int i = 0; i < 4; ++i) {
+            const int at = (own_start >> 2) + i;
+            word[i] = rows_of_warp + lane * kPitch + ((at & 4) + ((at + (lane >> 3)) & 3)) * 4;
+          }
+          uint4 carry = make_uint4(0u, 0u, 0u, 0u);  // what a turn leaves to the next
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              *reinterpret_cast<uint4*>(box + lane * 128 + ((k ^ (lane & 7)) << 4)) =
-                  Pack<float>::make(acc + 32 * c + 4 * k);
-            __syncwarp();
-            const int col = col0 + 32 * c + lane;
-            if (col < p.n) {
-#pragma unroll 4
-              for (int r = 0; r < left; ++r) {
-                const int64_t rr = row0 + r;
-                float v = f[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
-                if (res) v += to_f32(res[rr * p.ldr + col]);
-                out[rr * p.ldo + col] = from_f32<OutT>(v);
+          for (int t = 0; t < kBoxes; ++t) {
+            const uint32_t room = t % 2 * 32 * kPitch, rows_at = rows_of_warp + room, own = rows_at + lane * kPitch;
+            const int lo = t * 128, hi = t + 1 < kBoxes ? lo + 128 : lo + kPitch;  // bytes of the rows in this turn
+            if (res_rows) {
+              ok = __all_sync(0xFFFFFFFFu, mbar_wait(&res_bar[t], turn & 1, status)) && ok;
+              const int rs = start_of(residual_row());
+              uint4 u = load_shared4(own);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {  // four words of the row, out of two blocks
+                const uint4 next = load_shared4(own + 16 * c + 16);
+                uint32_t w[8] = {u.x, u.y, u.z, u.w, next.x, next.y, next.z, next.w};
+#pragma unroll
+                for (int i = 0; i < 6; ++i) w[i] = rs & 8 ? w[i + 2] : w[i];
+#pragma unroll
+                for (int i = 0; i < 5; ++i) w[i] = rs & 4 ? w[i + 1] : w[i];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  float* v = acc + (t * 32 + c * 4 + i) * kPer;
+                  if constexpr (kPer == 1) {
+                    v[0] += __uint_as_float(w[i]);
+                  } else {
+                    const uint32_t x = __funnelshift_r(w[i], w[i + 1], (rs & 2) * 8);
+                    const OutT* e = reinterpret_cast<const OutT*>(&x);
+                    v[0] += to_f32(e[0]);
+                    v[1] += to_f32(e[1]);
+                  }
+                }
+                u = next;
               }
+            } else {
+              __syncwarp();
+            }
+            if (t > 0) store_shared(own, carry);
+            uint32_t before = 0;
+#pragma unroll
+            for (int i = t > 0 && kPer == 2 ? -1 : 0; i < 32; ++i) {
+              uint32_t w;
+              if constexpr (kPer == 1) w = __float_as_uint(acc[t * 32 + i]);
+              else w = pack2(acc[t * 64 + 2 * i], acc[t * 64 + 2 * i + 1], OutT());
+              if (i >= 0)
+                store_shared(word[i & 3] + room + (i & ~3) * 4, kPer == 1 ? w : __funnelshift_l(before, w, (own_start & 2) * 8));
+              before = w;
+            }
+            if (kPer == 2 && t + 1 == kBoxes) store_shared(word[0] + room + 128, before >> 16);
+            if (t + 1 < kBoxes) carry = load_shared4(own + 128);
+            __syncwarp();
+            const bool tails = bytes + 15 >= lo && (bytes & ~15) < hi;  // some row may end here
+#pragma unroll
+            for (int r0 = 0; r0 < 32; r0 += 4) {
+              const int r = r0 + (lane >> 3), j = lane & 7;
+              OutT* to = out + static_cast<int64_t>(row0 + r) * p.ldo + col0;
+              const int start = start_of(to), end = row0 + r < p.m ? start + bytes : 0;
+              uint8_t* block = reinterpret_cast<uint8_t*>(to) - start;
+              const uint32_t from = rows_at + r * kPitch;
+              auto element = [&](int at) {
+                if (at < lo || at >= hi) return;
+                const uint32_t w = load_shared(from + ((at - lo) & ~15) + (((at >> 2) + (r0 >> 3)) & 3) * 4);
+                if constexpr (kPer == 1)
+                  *reinterpret_cast<uint32_t*>(block + at) = w;
+                else
+                  *reinterpret_cast<uint16_t*>(block + at) = static_cast<uint16_t>(w >> (at & 2) * 8);
+              };
+              if (lo + 16 * j >= start && lo + 16 * j + 16 <= end) {
+                const uint4 u = load_shared4(from + 16 * j);
+                const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+                *reinterpret_cast<uint4*>(block + lo + 16 * j) =
+                    make_uint4(x[(r0 >> 3) & 3], x[((r0 >> 3) + 1) & 3], x[((r0 >> 3) + 2) & 3], x[((r0 >> 3) + 3) & 3]);
+              }
+              const int inner = (start + 15) & ~15;  // the first block that the row begins
+              if (t == 0 && start + j * kSize < min(inner, end)) element(start + j * kSize);
+              if (tails) {
+                const int at = max(end & ~15, inner) + j * kSize;
+                if (at < end) element(at);
+              }
+            }
+            if (res_rows && t + 2 < kBoxes) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              fetch_rows(t + 2);
             }
           }
         }
@@ -598,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Stores have to finish before the CTA ends; so do the residual loads that
     // a wait that ran out left behind (with a limit: some were never issued).
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-    if (!ok && res_boxes)
+    if (!ok && (res_boxes || res_rows))
       for (int c = 0; c < kBoxes; ++c) mbar_wait_limit(&res_bar[c], turn & 1, status, kWaitLimitNs / 1000);
   }
 
@@ -663,7 +819,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using PL = Plan<BN, A_ROWS>;
   constexpr bool kCodes = sizeof(OutT) == 1;
   constexpr int kChunks = BN / 64;  // 32-column chunks of a thread's half
-  static_assert(!GATED || BN == 256, "the gated product needs 128 features of both weights");
+  static_assert(BN == (GATED ? 256 : 128), "a tile is 128 features, of both weights in the gated product");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + PL::kOffBar);
@@ -752,6 +908,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
+  // the residual of a warp's next row is on its way while a row is finished (m =
+  // 128, k = n = 768, a CTA per tile: 9.8 -> 7.5 us)
+  const int first = rank + split * (warp - 4);  // row
+  const OutT* res = GATED ? nullptr : static_cast<const OutT*>(p.residual);
+  Raw4<OutT> next;
+  if (warp >= 4 && res && first < rows)
+    next.load(res + static_cast<int64_t>(m0 + first) * p.ldr + f0 + lane * 4, p.n - f0 - lane * 4);
   __syncwarp();
   if (split > 1)
     cluster_sync();
@@ -783,7 +946,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return v;
     };
-    for (int r = rank + split * (warp - 4); r < rows; r += split * 8) {
+    for (int r = first; r < rows; r += split * 8) {
       const int64_t row = m0 + r;
       if constexpr (GATED) {
         // lane: features 4 lane .. 4 lane + 3 of the tile's 128
@@ -800,21 +963,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           store_codes4(static_cast<uint8_t*>(p.out) + row * p.ldo + col, p.n - col,
                        pack_e4m3x4(v.x * fac, v.y * fac, v.z * fac, v.w * fac));
         } else {
-          store4(static_cast<OutT*>(p.out) + row * p.ldo + col, p.n - col, p.vec_o, v);
+          store4(static_cast<OutT*>(p.out) + row * p.ldo + col, left, v);
         }
       } else {
-        const OutT* res = static_cast<const OutT*>(p.residual);
-#pragma unroll
-        for (int c = 0; c < BN / 128; ++c) {
-          const int col = f0 + c * 128 + lane * 4;
-          float4 rv = res ? load4(res + row * p.ldr + col, p.n - col, p.vec_r) : make_float4(0.f, 0.f, 0.f, 0.f);
-          const float4 v = total(r, c * 32 + lane);
-          rv.x += v.x;
-          rv.y += v.y;
-          rv.z += v.z;
-          rv.w += v.w;
-          store4(static_cast<OutT*>(p.out) + row * p.ldo + col, p.n - col, p.vec_o, rv);
+        const int col = f0 + lane * 4;
+        float4 v = total(r, lane);
+        if (res) {
+          const float4 x = next.value();
+          if (r + split * 8 < rows) next.load(res + (row + split * 8) * p.ldr + col, p.n - col);
+          v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
         }
+        store4(static_cast<OutT*>(p.out) + row * p.ldo + col, p.n - col, v);
       }
     }
   }
@@ -910,10 +1069,10 @@ cudaLaunchAttribute cluster_of(int n) {
 
 int clusters_of(int num_sms) { return std::max(1, num_sms / 2); }
 
-template <bool GATED, typename OutT>
+template <bool GATED, typename OutT, bool BOXES>
 cudaError_t launch_pair(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
-  constexpr auto kernel = pair::fp8_pair_kernel<GATED, OutT>;
-  cudaError_t e = allow_smem<kernel>(pair::Plan<GATED, OutT>::kSmem);
+  constexpr auto kernel = pair::fp8_pair_kernel<GATED, OutT, BOXES>;
+  cudaError_t e = allow_smem<kernel>(pair::Plan<GATED, OutT, BOXES>::kSmem);
   if (e != cudaSuccess) return e;
   CUtensorMap ta, tw, tu;
   if (!codes_map(&ta, p.a, p.m, p.k, p.lda, kRows) || !codes_map(&tw, p.w, p.n, p.k, p.ldw, 64) ||
@@ -927,18 +1086,16 @@ cudaError_t launch_pair(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
   const int clusters = static_cast<int>(std::min<int64_t>(tiles, clusters_of(num_sms)));
   // results by TMA boxes where rows (and the residual's) start at multiples of 16 bytes
   CUtensorMap to = ta, tr = ta;
-  bool boxes = false;
   if constexpr (sizeof(OutT) == 1) {
     if (!codes_map(&to, static_cast<const uint8_t*>(p.out), p.m, p.n, p.ldo, 32, 64)) return cudaErrorInvalidValue;
-  } else {
-    boxes = p.box_o && (!p.residual || p.box_r);
-    if (boxes && (!values_map<OutT>(&to, p.out, p.m, p.n, p.ldo) ||
-                  (p.residual && !values_map<OutT>(&tr, p.residual, p.m, p.n, p.ldr))))
+  } else if constexpr (BOXES) {
+    if (!values_map<OutT>(&to, p.out, p.m, p.n, p.ldo) ||
+        (p.residual && !values_map<OutT>(&tr, p.residual, p.m, p.n, p.ldr)))
       return cudaErrorInvalidValue;
   }
   const cudaLaunchAttribute attr = cluster_of(2);
-  return launch_pdl(kernel, dim3(2 * clusters), dim3(kThreads), pair::Plan<GATED, OutT>::kSmem, st, &attr, 1, ta, tw, tu, to, tr, p,
-                    boxes);
+  return launch_pdl(kernel, dim3(2 * clusters), dim3(kThreads), pair::Plan<GATED, OutT, BOXES>::kSmem, st, &attr, 1, ta, tw, tu, to, tr,
+                    p);
 }
 
 template <bool GATED, typename OutT, int BN, int A_ROWS>
@@ -1003,7 +1160,8 @@ cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
   // start and an end that grow with its rows, and its blocks one after the
   // other; a join over a cluster costs extra; more tiles than SMs go in rounds.
   // A pair's round is cheaper per element but starts slower, and rows off the
-  // 16-byte boundary cost it an element-wise way out.  Measured with 768 <= k <=
+  // 16-byte boundary cost it more than the single tile, whose CTAs also share the
+  // residual's rows.  Measured with 768 <= k <=
   // 8192, 1 <= m <= 4096; at m = 128, k = 768, n = 2304: 6.1 / 6.8 / 5.6 / 6.5 us
   // with 1, 2, 4, 8 CTAs a tile and 6.8 on pairs.
   const Cost c = GATED ? Cost{2.8f, 4.2f, 0.46f, 0.6f, 2.8f, 1.8f, 0.45f} : Cost{2.05f, 1.95f, 0.32f, 0.65f, 4.0f, 1.0f, 0.42f};
@@ -1011,8 +1169,10 @@ cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
   constexpr int kPairFeat = GATED ? 128 : 256;
   const int64_t pairs = static_cast<int64_t>((p.m + 2 * kRows - 1) / (2 * kRows)) * ((p.n + kPairFeat - 1) / kPairFeat);
   const bool off = sizeof(OutT) > 1 && !(p.box_o && (!p.residual || p.box_r));
+  const float pair_off = !off ? 0.0f : (p.residual ? 3.2f : 1.3f) * (sizeof(OutT) == 4 ? 1.6f : 1.0f);
+  const float tile_res = !p.residual ? 0.0f : rows * (off ? 3.0f : 1.2f) * (sizeof(OutT) == 4 ? 2.0f : 1.0f);
   float best = c.pair_start + static_cast<float>((pairs + clusters_of(num_sms) - 1) / clusters_of(num_sms)) *
-                                  (c.pair_round + c.pair_block * kblocks + (off ? 3.5f : 0.0f));
+                                  (c.pair_round + c.pair_block * kblocks + pair_off);
   constexpr auto kernel = tile::fp8_tile_kernel<GATED, OutT, BN, kRows>;
   constexpr int kSmem = tile::Plan<BN, kRows>::kSmem;
   if (cudaError_t e = allow_smem<kernel>(kSmem); e != cudaSuccess) return e;
@@ -1020,17 +1180,18 @@ cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
   for (int s = 1; s <= 8 && s <= kblocks; s *= 2) {
     const int fit = resident_ctas<kernel>(s, kSmem, num_sms);
     const float rounds = static_cast<float>((tiles * s + fit - 1) / fit);
-    const float t = rounds * (c.tile + c.tile_rows * rows + c.block * static_cast<float>((kblocks + s - 1) / s) +
+    const float t = rounds * (c.tile + c.tile_rows * rows + tile_res / s + c.block * static_cast<float>((kblocks + s - 1) / s) +
                               (s > 1 ? c.join : 0.0f));
     if (t < best) {
       best = t;
       split = s;
     }
   }
-#ifdef WC_FP8_SWEEP
-  if (const char* f = getenv("WC_FP8_FORCE")) split = std::min<int>(atoi(f), kblocks);
-#endif
-  if (split == 0) return launch_pair<GATED, OutT>(p, num_sms, st);
+  if (split == 0) {
+    if constexpr (sizeof(OutT) > 1)
+      if (off) return launch_pair<GATED, OutT, false>(p, num_sms, st);
+    return launch_pair<GATED, OutT, true>(p, num_sms, st);
+  }
   return p.m <= 32 ? launch_tile<GATED, OutT, BN, 32>(p, split, st) : launch_tile<GATED, OutT, BN, kRows>(p, split, st);
 }
 

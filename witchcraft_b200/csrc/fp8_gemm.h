@@ -15,8 +15,7 @@ struct Fp8GemmParams {
   int64_t lda, ldw, ldup, ldsa, ldsw, ldsup, ldr, ldo, ldos;
   int m, n, k;
   int act;                           // WC_ACT_*, gated only
-  bool vec_o, vec_r;                 // output / residual rows aligned to four elements
-  bool box_o, box_r;                 // ... and to 16 bytes
+  bool box_o, box_r;                 // rows of 16-byte blocks: whole ones of the output, aligned ones of the residual
   uint32_t* status;                  // wait timeouts; null: the library's own word
 };
 
