@@ -80,6 +80,17 @@ def test_weight(n, k, dtype):
     check_codes(codes, scales, w.double(), rows=128)
 
 
+@pytest.mark.parametrize("dtype", TYPES.values(), ids=TYPES)
+def test_codes_are_those_of_the_rounded_quotient(dtype):
+    """x / scale in f32, rounded, then to e4m3: ties between two codes, which
+    16-bit values meet often, included."""
+    x = randn(2000, 700, seed=3, dtype=dtype)
+    x[:, ::128] = 448.0 * 2.0 ** torch.randint(-8, 8, (2000, 6), generator=gen(4), device="cuda")  # scales that are powers of two
+    for codes, scales, rows in ((*fp8.quantize(x), 1), (*fp8.quantize_weight(x), 128)):
+        s = scales.repeat_interleave(rows, 0)[:2000].repeat_interleave(128, 1)[:, :700]
+        assert torch.equal(codes.float(), (x.float() / s).to(torch.float8_e4m3fn).float())
+
+
 def test_rows_special_values():
     x = torch.zeros(9, 256, device="cuda")
     x[1] = 1e-40                    # denormal

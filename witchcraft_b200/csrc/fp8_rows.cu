@@ -188,12 +188,37 @@ __device__ __forceinline__ void put8(T* p, int left, const Eight& x) {
     }
   }
 }
-// The codes of eight values times f.
-template <bool VEC, bool APART>
-__device__ __forceinline__ void put_codes8(uint8_t* p, int left, const Eight& x, float f) {
+// The codes of eight values over their scale s, f = 1 / s: the product with f
+// corrected by its remainder (Markstein's step), so the code is that of the
+// rounded quotient and a tie between two codes stays one.  (With the product
+// alone, one code in 10^5 of 16-bit values is the other neighbour of a tie.)
+// Two at a time where registers allow (rows of f16, m = 16384, k = 768: 8.4 ->
+// 8.0 us; 7.7 without the correction); the norm, which is out of them, takes one
+// (bf16, m = 4095, k = 5000: 32.9 us, 33.7 by twos).
+template <bool TWO>
+__device__ __forceinline__ float2 quotients(float x, float y, float s, float f) {
+  float2 q;
+  if constexpr (TWO) {
+    asm("{\n\t.reg .b64 v, s, f, q, r;\n\t"
+        "mov.b64 v, {%2, %3};\n\tmov.b64 s, {%4, %4};\n\tmov.b64 f, {%5, %5};\n\t"
+        "mul.rn.f32x2 q, v, f;\n\tfma.rn.f32x2 r, q, s, v;\n\tfma.rn.f32x2 q, r, f, q;\n\t"
+        "mov.b64 {%0, %1}, q;\n\t}"
+        : "=f"(q.x), "=f"(q.y)
+        : "f"(x), "f"(y), "f"(-s), "f"(f));
+  } else {
+    q = make_float2(x * f, y * f);
+    q.x = __fmaf_rn(__fmaf_rn(-q.x, s, x), f, q.x);
+    q.y = __fmaf_rn(__fmaf_rn(-q.y, s, y), f, q.y);
+  }
+  return q;
+}
+template <bool VEC, bool APART, bool TWO>
+__device__ __forceinline__ void put_codes8(uint8_t* p, int left, const Eight& x, float s, float f) {
   constexpr int d = kSecond<APART>;
-  const uint32_t a = pack_e4m3x4(x.v[0] * f, x.v[1] * f, x.v[2] * f, x.v[3] * f);
-  const uint32_t b = pack_e4m3x4(x.v[4] * f, x.v[5] * f, x.v[6] * f, x.v[7] * f);
+  float2 q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = quotients<TWO>(x.v[2 * i], x.v[2 * i + 1], s, f);
+  const uint32_t a = pack_e4m3x4(q[0].x, q[0].y, q[1].x, q[1].y), b = pack_e4m3x4(q[2].x, q[2].y, q[3].x, q[3].y);
   if (!APART && left >= 8) {
     *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
   } else if (!VEC) {
@@ -206,11 +231,11 @@ __device__ __forceinline__ void put_codes8(uint8_t* p, int left, const Eight& x,
 }
 // Quantises one unit of a row: this lane's eight values, `left` columns of the
 // row being left from its first one on.
-template <bool VEC, bool APART>
+template <bool VEC, bool APART, bool TWO>
 __device__ __forceinline__ void put_unit(uint8_t* codes, float* scale, int lane, int left, const Eight& x) {
   const float s = fp8_scale(half_warp_max_nan(max_abs(x)));
   if ((lane & 15) == 0 && left > 0) *scale = s;
-  put_codes8<VEC, APART>(codes, left, x, fp8_factor(s));
+  put_codes8<VEC, APART, TWO>(codes, left, x, s, fp8_factor(s));
 }
 
 // Blocks are independent: one warp per kHeld units of a row, all loads issued
@@ -236,7 +261,7 @@ __global__ void __launch_bounds__(32 * kWarps) fp8_rows_kernel(const __grid_cons
 #pragma unroll
   for (int g = 0; g < kHeld; ++g) {
     if (left - g * kUnit + run <= 0) break;  // the whole unit is past the row
-    put_unit<VEC, kApart>(codes + g * kUnit, scales + g * 2, lane, left - g * kUnit, widen(v[g]));
+    put_unit<VEC, kApart, true>(codes + g * kUnit, scales + g * 2, lane, left - g * kUnit, widen(v[g]));
   }
 }
 
@@ -299,7 +324,7 @@ __global__ void __launch_bounds__(32 * kWarps, 5) fp8_rmsnorm_kernel(const __gri
     const Eight w = widen(get8<VEC, kApart>(p.w + off + g * kStep, left));
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[g].v[i] *= inv * w.v[i];
-    put_unit<VEC, kApart>(codes + g * kStep, scales + g * (kStep / kFp8Block), lane, left, v[g]);
+    put_unit<VEC, kApart, false>(codes + g * kStep, scales + g * (kStep / kFp8Block), lane, left, v[g]);
   }
 }
 
@@ -348,7 +373,7 @@ __global__ void __launch_bounds__(32 * kWarps) fp8_rmsnorm_wide_kernel(const __g
     const Eight w = widen(get8<VEC, kApart>(p.w + off + c, left));
 #pragma unroll
     for (int i = 0; i < 8; ++i) v.v[i] *= inv * w.v[i];
-    put_unit<VEC, kApart>(p.codes + row * p.ldc + off + c, p.scales + row * p.lds + (off + c) / kFp8Block, lane, left, v);
+    put_unit<VEC, kApart, false>(p.codes + row * p.ldc + off + c, p.scales + row * p.lds + (off + c) / kFp8Block, lane, left, v);
   }
 }
 
@@ -382,7 +407,7 @@ __global__ void __launch_bounds__(32 * kWarps) fp8_weight_kernel(const __grid_co
 #pragma unroll
   for (int t = 0; t < kTurns; ++t) {
     const int64_t row = row0 + 2 * kWarps * t;
-    if (row < p.m) put_codes8<VEC, kApart>(p.codes + row * p.ldc + col, left, widen(v[t]), f);
+    if (row < p.m) put_codes8<VEC, kApart, true>(p.codes + row * p.ldc + col, left, widen(v[t]), s, f);
   }
 }
 
