@@ -8,8 +8,13 @@
 // values (16 bytes) and lie 64 columns apart for f32 (two accesses of 16 bytes
 // of which each covers whole lines: norm m = 16384, k = 768: 29.4 -> 27.1 us).
 // VEC: every row is aligned to eight elements and k is a multiple of eight, so
-// an access is either whole or absent; the other form takes the edge element by
-// element.
+// an access is either whole or absent; the other form takes rows that start
+// anywhere, in pieces or element by element.
+//
+// Measured (device time, inputs from DRAM): norm f32 16384 x 768 with an f16
+// residual 26.2 us or 5.3 TB/s, bf16 4095 x 5000 32.9 us or 4.4 TB/s; rows f16
+// 16384 x 768 8.0 us or 4.8 TB/s; weight f32 2048 x 768 3.7 us, 32 rows of norm
+// 3.3 us, both latency.
 #include "fp8.cuh"
 #include "fp8_rows.h"
 
@@ -267,7 +272,7 @@ __global__ void __launch_bounds__(32 * kWarps) fp8_rows_kernel(const __grid_cons
 
 // One row by WPR warps, its kHeld units per warp in registers between the sum
 // of squares and the scaling (rows up to WPR * kHeld * 256 columns).  Five CTAs
-// an SM at 48 registers (norm m = 16384, k = 768: 27.1 us with four, 26.1 with
+// an SM at 48 registers (norm m = 16384, k = 768: 27.1 us with four, 26.2 with
 // five, 34.3 with six, which spill): the loads of one row overlap the
 // arithmetic of the others.
 template <typename TX, typename TD, bool DELTA, bool VEC, int WPR>
