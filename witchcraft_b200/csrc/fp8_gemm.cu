@@ -228,8 +228,8 @@ __device__ __forceinline__ bool sum_blocks(float (&acc)[32 * CHUNKS], Scales& sc
         tmem_ld32_issue(at + 32 * (c + 1), r[(c + 1) & 1]);
       } else {
         tc_fence_before();
-    __syncwarp();
-    read(ring.i % BUFS);
+        __syncwarp();
+        read(ring.i % BUFS);
       }
       add(c);
     }
