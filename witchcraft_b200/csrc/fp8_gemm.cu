@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      ++turn;
+      if (ok || kCodes) ++turn;  // else what is left of this tile is waited for below
     }
     // Stores have to finish before the CTA ends; so do the residual loads that
     // a wait that ran out left behind (with a limit: some were never issued).
