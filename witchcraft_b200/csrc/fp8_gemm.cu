@@ -495,7 +495,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // the same for rows off the 16-byte boundary: the 16-byte blocks that hold
       // 128 bytes of a row from its start's block on, a bulk copy per row (what a
-      // block holds of other rows is not used)
+      // block holds of other rows is not used, and what the first and the last
+      // block of the whole residual hold is read by elements)
       const int res_bytes = row0 + lane < p.m ? max(0, min(p.n - col0, kFeat / 2)) * static_cast<int>(sizeof(OutT)) : 0;
       auto residual_row = [&] {
         return static_cast<const OutT*>(p.residual) + static_cast<int64_t>(row0 + lane) * p.ldr + col0;
@@ -503,16 +504,35 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto fetch_rows = [&](int t) {
         const uint8_t* from = reinterpret_cast<const uint8_t*>(residual_row());
         const int start = static_cast<int>(reinterpret_cast<uintptr_t>(from) & 15);
-        const int end = res_bytes ? (start + res_bytes + 15) & ~15 : 0;
-        const int size = max(0, min(end - t * 128, kPitch));
+        const int end = res_bytes ? (start + res_bytes + 15) & ~15 : 0, row = row0 + lane;
+        // the blocks that the whole residual starts and ends in are not read past it
+        const bool first = row == 0 && col0 == 0 && start != 0;
+        const bool last = row == p.m - 1 && p.n - col0 <= kFeat / 2 && (start + res_bytes) % 16 != 0;
+        const int lo = t * 128 + (first && t == 0 ? 16 : 0);
+        const int hi = min(last ? end - 16 : end, t * 128 + kPitch);
+        const int size = max(0, hi - lo);
+        const uint32_t to = smem_u32(box) + (t % 2 * 32 + lane) * kPitch - t * 128;
+        auto elements = [&](int block) {
+          using Bits = std::conditional_t<sizeof(OutT) == 4, uint32_t, uint16_t>;
+#pragma unroll 1
+          for (int at = max(block, start); at < min(block + 16, start + res_bytes); at += sizeof(OutT)) {
+            const Bits v = *reinterpret_cast<const Bits*>(from - start + at);
+            if constexpr (sizeof(OutT) == 4)
+              store_shared(to + at, static_cast<uint32_t>(v));
+            else
+              asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + at), "h"(v) : "memory");
+          }
+        };
+        if (res_bytes && first && t == 0) elements(0);
+        if (res_bytes && last && end - 16 >= t * 128 && end - 16 < t * 128 + kPitch) elements(end - 16);
         const uint32_t sum = __reduce_add_sync(0xFFFFFFFFu, static_cast<uint32_t>(size));
         if (lane == 0) mbar_arrive_expect_tx(&res_bar[t], sum);
         __syncwarp();
         if (size > 0)
           asm volatile(
               "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                  smem_u32(box + (t % 2 * 32 + lane) * kPitch)),
-              "l"(from - start + t * 128), "r"(size), "r"(smem_u32(&res_bar[t]))
+                  to + lo),
+              "l"(from - start + lo), "r"(size), "r"(smem_u32(&res_bar[t]))
               : "memory");
       };
       if (res_rows) {
