@@ -341,6 +341,29 @@ struct Plan {
   static_assert(2 * 2 * kRows * 4 <= kBoxBytes, "maxima of two tiles");
 };
 
+// Of the stores that a warp committed, how many may still be reading their room
+// when box c of a tile is written into room c % bufs.  The rooms start over with
+// every tile, so they are not used in turn across tiles: the first box waits for
+// all that the tile before stored (a whole sum ago), and the boxes that reuse a
+// room of their own tile for the one that was in it.  kAnyStores: no wait.
+constexpr int kAnyStores = 1 << 20;
+__host__ __device__ constexpr int stores_in_flight(int c, int bufs) {
+  return c == 0 ? 0 : c < bufs ? kAnyStores : bufs - 1;
+}
+// Several tiles of `boxes` boxes, a store (and group) each: whether every box
+// finds its room read.
+constexpr bool rooms_are_read(int boxes, int bufs) {
+  int last[8] = {-1, -1, -1, -1, -1, -1, -1, -1}, read = 0, committed = 0;  // groups [0, read) are known to be read
+  for (int tile = 0; tile < 4; ++tile)
+    for (int c = 0; c < boxes; ++c) {
+      if (committed - stores_in_flight(c, bufs) > read) read = committed - stores_in_flight(c, bufs);
+      if (last[c % bufs] >= read) return false;
+      last[c % bufs] = committed++;
+    }
+  return true;
+}
+static_assert(rooms_are_read(1, 2) && rooms_are_read(4, 3), "plans whose boxes go one at a time");
+
 __device__ __forceinline__ uint32_t load_shared(uint32_t at) {
   uint32_t v;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
@@ -626,6 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // and written by TMA stores, which clip what lies outside.  Two of
           // two boxes go together, with one fence; of four, one at a time.
           constexpr int kN = Pack<OutT>::kN, kTogether = kBoxes == 2 ? 2 : 1;
+          static_assert(kTogether == 2 ? kBoxes == 2 && kBufs >= 2 : rooms_are_read(kBoxes, kBufs), "");
 #pragma unroll
           for (int c0 = 0; c0 < kBoxes; c0 += kTogether) {
             if (res_boxes) {
@@ -633,11 +657,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int c = c0; c < c0 + kTogether; ++c)
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait(&res_bar[c], turn & 1, status)) && ok;
             } else {
+              constexpr int kBack = kBufs - 1;
               if (lane == 0) {
-                if (kTogether == 2)
+                if (stores_in_flight(c0, kBufs) == 0)
                   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                else
-                  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kBufs - 1) : "memory");
+                else if (stores_in_flight(c0, kBufs) == kBack)
+                  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kBack) : "memory");
               }
               __syncwarp();
             }
