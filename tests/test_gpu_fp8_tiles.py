@@ -4,7 +4,7 @@ one.  Against 64 bits, with the bounds of test_gpu_fp8.py."""
 import pytest
 import torch
 
-from test_gpu_fp8 import ROUND, TYPES, gated64, operands, product64
+from test_gpu_fp8 import ROUND, TYPES, U, gated64, operands, product64, randn
 from witchcraft_b200 import fp8
 
 pytestmark = pytest.mark.gpu
@@ -37,3 +37,22 @@ def test_boxes_of_gated_results(m, k, n, dtype):
     want, err = gated64(a, sa, gate, up, "gelu")
     for _ in range(3):
         assert near(fp8.gated_matmul(a, sa, *gate, *up, out_dtype=dtype), want, err)
+
+
+@pytest.mark.parametrize("m,n", [(20001, 3), (20001, 1), (8002, 129), (8002, 257), (8002, 130)])
+@pytest.mark.parametrize("dtype", TYPES.values(), ids=TYPES)
+@pytest.mark.parametrize("offset", [0, 2])
+def test_residual_of_adjoining_rows(m, n, dtype, offset):
+    """Rows without a gap, off the 16-byte boundary, some of them several to a
+    block: the residual's own values and nothing of its neighbours."""
+    a, sa, [(w, sw)] = operands(m, 140, n, seed=n)
+    flat = torch.full((m * n + 16,), float("nan"), dtype=dtype, device="cuda")
+    res = flat[4 + offset:4 + offset + m * n].view(m, n)
+    res.copy_(randn(m, n, seed=1, dtype=dtype))
+    want, err = product64(a, sa, w, sw)
+    want = want + res.double()
+    err = err + U * want.abs()
+    assert near(fp8.matmul(a, sa, w, sw, residual=res), want, err)
+    fp8.matmul(a, sa, w, sw, residual=res, out=res)
+    assert near(res, want, err)
+    assert torch.isnan(flat[:4 + offset]).all() and torch.isnan(flat[4 + offset + m * n:]).all()

@@ -40,6 +40,7 @@
 #include "cluster.cuh"
 #include "fp8.cuh"
 #include "fp8_gemm.h"
+#include "fp8_span.h"
 
 #include <algorithm>
 #include <mutex>
@@ -317,7 +318,7 @@ namespace pair {
 constexpr int kBN = 256;
 constexpr int kStageBytes = kABytes + 128 * kFp8Block;
 constexpr int kBoxBytes = 32 * 128;  // 32 rows x 128 bytes of results (or of the residual)
-constexpr int kPitch = 128 + 16;     // of such a row that starts inside a block of 16 bytes
+constexpr int kPitch = kTurnRoom;    // of such a row that starts inside a block of 16 bytes
 
 // Shared memory: operand stages, then boxes of results for each epilogue warp
 // (a warp's results are four boxes of f32 or two of 16-bit values).
@@ -518,23 +519,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // the same for rows off the 16-byte boundary: the 16-byte blocks that hold
       // 128 bytes of a row from its start's block on, a bulk copy per row (what a
-      // block holds of other rows is not used, and what the first and the last
-      // block of the whole residual hold is read by elements)
+      // block holds of other rows is not used, and what a block that reaches out
+      // of the residual holds of it is read by elements)
       const int res_bytes = row0 + lane < p.m ? max(0, min(p.n - col0, kFeat / 2)) * static_cast<int>(sizeof(OutT)) : 0;
       auto residual_row = [&] {
         return static_cast<const OutT*>(p.residual) + static_cast<int64_t>(row0 + lane) * p.ldr + col0;
       };
       auto fetch_rows = [&](int t) {
         const uint8_t* from = reinterpret_cast<const uint8_t*>(residual_row());
+        const OutT* base = static_cast<const OutT*>(p.residual);
+        const ResidualSpan span =
+            residual_span(reinterpret_cast<uintptr_t>(from), res_bytes, reinterpret_cast<uintptr_t>(base),
+                          reinterpret_cast<uintptr_t>(base + static_cast<int64_t>(p.m - 1) * p.ldr + p.n), t);
         const int start = static_cast<int>(reinterpret_cast<uintptr_t>(from) & 15);
-        const int end = res_bytes ? (start + res_bytes + 15) & ~15 : 0, row = row0 + lane;
-        // the blocks that the whole residual starts and ends in are not read past it
-        const bool first = row == 0 && col0 == 0 && start != 0;
-        const bool last = row == p.m - 1 && p.n - col0 <= kFeat / 2 && (start + res_bytes) % 16 != 0;
-        const int lo = t * 128 + (first && t == 0 ? 16 : 0);
-        const int hi = min(last ? end - 16 : end, t * 128 + kPitch);
-        const int size = max(0, hi - lo);
-        const uint32_t to = smem_u32(box) + (t % 2 * 32 + lane) * kPitch - t * 128;
+        const int lo = span.lo, size = max(0, span.hi - span.lo);
+        const uint32_t to = smem_u32(box) + (t % 2 * 32 + lane) * kPitch - t * kTurnBytes;
         auto elements = [&](int block) {
           using Bits = std::conditional_t<sizeof(OutT) == 4, uint32_t, uint16_t>;
 #pragma unroll 1
@@ -546,8 +545,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + at), "h"(v) : "memory");
           }
         };
-        if (res_bytes && first && t == 0) elements(0);
-        if (res_bytes && last && end - 16 >= t * 128 && end - 16 < t * 128 + kPitch) elements(end - 16);
+        if (span.head) elements(0);
+        if (span.tail) elements(span.last);
         const uint32_t sum = __reduce_add_sync(0xFFFFFFFFu, static_cast<uint32_t>(size));
         if (lane == 0) mbar_arrive_expect_tx(&res_bar[t], sum);
         __syncwarp();
