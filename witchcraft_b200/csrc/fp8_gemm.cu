@@ -87,6 +87,16 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// Waits for a barrier of the operand ring or of the partials: on pairs of SMs the
+// other CTA's loads, its epilogue or the even CTA's MMAs arrive there.
+template <bool PAIR>
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  if constexpr (PAIR)
+    return mbar_wait_cluster_relaxed(bar, parity, status);
+  else
+    return mbar_wait(bar, parity, status);
+}
+
 // The MMA warp's loop over `steps` blocks: STAGES operand stages of
 // STAGE_BYTES (A, then B) and BUFS partials of BN columns.  The whole warp
 // runs it and one lane issues, so that descriptors stay in uniform registers:
@@ -101,8 +111,9 @@ __device__ __forceinline__ void mma_loop(uint32_t tmem, uint32_t idesc, uint32_t
   for (uint32_t i = 0; i < steps; ++i) {
     const uint32_t buf = i % BUFS;
     const bool ok =
-        mbar_wait(&full[s], round & 1, status) && mbar_wait(&acc_empty[buf], ((i / BUFS) & 1) ^ 1, status);
+        ring_wait<PAIR>(&full[s], round & 1, status) && ring_wait<PAIR>(&acc_empty[buf], ((i / BUFS) & 1) ^ 1, status);
     if (!__all_sync(0xFFFFFFFFu, ok)) return;  // one way out for the whole warp
+    if (PAIR) acquire_cluster_shared();  // operands
     tc_fence_after();
     const uint64_t a = a0 + s * (STAGE_BYTES >> 4), b = b0 + s * (STAGE_BYTES >> 4);
     const uint32_t d = tmem + buf * BN;
@@ -202,7 +213,7 @@ struct Ring {
 // the next block's first columns in flight across the loop's end made the
 // whole product twice as slow.  `read(buf)` once a partial is in registers.
 // False if a wait ran out.
-template <bool GATED, int CHUNKS, int STAGES, int BUFS, int BN, typename Read>
+template <bool PAIR, bool GATED, int CHUNKS, int STAGES, int BUFS, int BN, typename Read>
 __device__ __forceinline__ bool sum_blocks(float (&acc)[32 * CHUNKS], Scales& sc, int blocks, int step, uint32_t taddr,
                                            uint64_t* done, Ring<STAGES>& ring, uint32_t* status, Read read) {
   static_assert(CHUNKS == 2 || CHUNKS == 4, "two register sets");
@@ -213,7 +224,7 @@ __device__ __forceinline__ bool sum_blocks(float (&acc)[32 * CHUNKS], Scales& sc
   for (int left = blocks; left > 0; --left) {
     const float s0 = sc.va * sc.vw, s1 = GATED ? sc.va * sc.vu : s0;
     if (left > 1) fetch_scales<GATED>(sc, step);
-    if (!__all_sync(0xFFFFFFFFu, mbar_wait(&done[ring.stage], ring.parity, status))) return false;
+    if (!__all_sync(0xFFFFFFFFu, ring_wait<PAIR>(&done[ring.stage], ring.parity, status))) return false;
     tc_fence_after();
     const uint32_t at = taddr + ring.i % BUFS * BN;
     auto add = [&](int c) {
@@ -446,7 +457,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int f0 = (tile % n_tiles) * kFeat + rank * (kFeat / 2);
         for (int kb = 0; kb < kblocks; ++kb, ++i) {
           const uint32_t s = i % kStages;
-          if (!(ok = mbar_wait(&done[s], ((i / kStages) & 1) ^ 1, status))) break;
+          if (!(ok = ring_wait<true>(&done[s], ((i / kStages) & 1) ^ 1, status))) break;
+          acquire_cluster_shared();
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
           uint8_t* sa = smem + s * kStageBytes;
           const uint32_t bar = map_to_rank(&full[s], 0);
@@ -566,10 +578,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint8_t*>(residual_row()) + c));
       }
       float acc[128];
-      ok = ok && sum_blocks<GATED, 4, kStages, 2, kBN>(
+      ok = ok && sum_blocks<true, GATED, 4, kStages, 2, kBN>(
           acc, sc, kblocks, 1, tlane, done, ring, status,
           [&](uint32_t buf) {
-            if (lane == 0) mbar_arrive_remote(empty0 + buf * 8);
+            if (lane == 0) mbar_arrive_remote_relaxed(empty0 + buf * 8);
           });
       if (!ok && !kCodes) break;
       sc = open_tile(tile + tile_step);  // arrives while this tile is written
@@ -947,7 +959,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float acc[32 * kChunks];
       Ring<PL::kStages> ring;
       fetch_scales<GATED>(sc, split);
-      sum_blocks<GATED, kChunks, PL::kStages, PL::kBufs, BN>(
+      sum_blocks<false, GATED, kChunks, PL::kStages, PL::kBufs, BN>(
           acc, sc, blocks, split, tlane, done, ring, status,
           [&](uint32_t buf) {
             if (lane == 0) mbar_arrive(&acc_empty[buf]);
