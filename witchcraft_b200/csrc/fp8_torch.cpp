@@ -5,6 +5,7 @@
 // loaded, so there is one instance of it.
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -41,7 +42,18 @@ std::string shape_of(const Tensor& t) {
 }
 std::string shape(int64_t r, int64_t c) { return "(" + std::to_string(r) + ", " + std::to_string(c) + ")"; }
 
+// Nothing here has a gradient: results would leave the graph without a word.
+void no_grad(const Tensor& t, const char* name) {
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    refuse(std::string(name) + " requires grad, and the 8-bit operators have no gradient; call them under torch.no_grad()");
+}
+// What autograd saved of `out` is another value now.
+void written(const Tensor& out) {
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
+
 void matrix(const Tensor& t, const char* name, const Tensor& like) {
+  no_grad(t, name);
   if (!t.is_cuda() || t.dim() != 2 || (t.stride(1) != 1 && t.size(1) > 1))
     refuse(std::string(name) + " must be a CUDA matrix with contiguous rows");
   if (t.get_device() != like.get_device())
@@ -147,6 +159,7 @@ py::tuple rmsnorm(const Tensor& x, const Tensor& weight, double eps, const std::
   const int code = values(x, "x", x);
   columns(x, "x");
   const int64_t m = x.size(0), k = x.size(1);
+  no_grad(weight, "weight");
   if (weight.scalar_type() != at::kFloat || weight.dim() != 1 || weight.size(0) != k || !weight.is_cuda() ||
       weight.get_device() != x.get_device() || (weight.stride(0) != 1 && k > 1))
     refuse("weight must be " + std::to_string(k) + " contiguous float32 values on " + x.device().str());
@@ -169,6 +182,7 @@ py::tuple rmsnorm(const Tensor& x, const Tensor& weight, double eps, const std::
                       delta ? sum.data_ptr() : nullptr, delta ? ld(sum) : 0, floats(weight), m, k,
                       static_cast<float>(eps), codes.data_ptr(), codes_ld(codes), floats(scales), scales.size(1),
                       stream_of(x)));
+  if (out) written(*out);
   return delta ? py::make_tuple(sum, codes, scales) : py::make_tuple(codes, scales);
 }
 
@@ -202,6 +216,7 @@ Tensor matmul(const Tensor& a, const Tensor& a_scales, const Tensor& w, const Te
     check(api.matmul(a.data_ptr(), codes_ld(a), floats(a_scales), ld(a_scales), m, k, w.data_ptr(), codes_ld(w),
                      floats(w_scales), ld(w_scales), n, residual ? residual->data_ptr() : nullptr,
                      residual ? ld(*residual) : 0, y.data_ptr(), code, ld(y), stream_of(a)));
+  if (out) written(*out);
   return y;
 }
 

@@ -12,7 +12,8 @@ one per 128 x 128 block.  A feed-forward block reads
 
 with each weight once through `quantize_weight`.  Everything runs on the
 current stream of the tensors' device; results are new tensors unless `out` is
-given.  (No counterpart in the reference, whose layers run in f32.)
+given.  For inference: the operators have no gradient and refuse tensors that
+require grad where grad mode is on.  (No counterpart in the reference, whose layers run in f32.)
 """
 from __future__ import annotations
 
