@@ -5,7 +5,8 @@ Every CUDA translation unit is compiled for sm_100a only
 The library links the CUDA runtime statically and reaches the driver's
 cuTensorMapEncodeTiled through cudaGetDriverEntryPointByVersion, so it needs
 no libcuda at link time and no torch at all.  The torch binding of the 8-bit
-operators is a second, small library, `witchcraft_b200/_fp8_torch.so`.
+operators is a second, small library, `witchcraft_b200/_fp8_torch.so`, built
+where torch with CUDA is installed and again for another version of it.
 
 Usage: python -m witchcraft_b200.build   (or witchcraft_b200.build.build())
 """
@@ -78,21 +79,31 @@ def build(verbose: bool = False, force: bool = False) -> str:
     return LIB
 
 
-def build_torch_binding(force: bool = False) -> str:
-    """The torch binding of the 8-bit operators (witchcraft_b200/fp8.py); the
-    library itself needs no torch."""
+def build_torch_binding(force: bool = False) -> str | None:
+    """The torch binding of the 8-bit operators (witchcraft_b200/fp8.py), or
+    None without torch or with one built without CUDA: the library itself needs
+    neither."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    if torch.version.cuda is None:
+        return None
+    import sysconfig
     src = os.path.join(CSRC, "fp8_torch.cpp")
     header = os.path.join(os.path.dirname(HERE), "include", "wc_fp8.h")
-    if force or _stale(TORCH_BINDING, [src, header]):
-        import sysconfig
-
-        import torch
+    stamp = os.path.join(BUILD_DIR, "fp8_torch.version")  # what the binding was built for
+    version = f"torch {torch.__version__}, python {sysconfig.get_config_var('SOABI')}"
+    built_for = open(stamp).read() if os.path.exists(stamp) else ""
+    if force or built_for != version or _stale(TORCH_BINDING, [src, header]):
         from torch.utils.cpp_extension import include_paths, library_paths
         inc = [f"-I{d}" for d in include_paths()] + [f"-I{sysconfig.get_paths()['include']}", "-I/usr/local/cuda/include"]
         abi = int(torch.compiled_with_cxx11_abi())
         _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *inc, src, "-o",
               TORCH_BINDING, *[f"-L{d}" for d in library_paths()], "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
               "-ltorch_python"])
+        with open(stamp, "w") as f:
+            f.write(version)
     return TORCH_BINDING
 
 
