@@ -614,8 +614,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            w[e] = pack_e4m3x4(acc[16 * c + 4 * e] * fac, acc[16 * c + 4 * e + 1] * fac, acc[16 * c + 4 * e + 2] * fac,
-                               acc[16 * c + 4 * e + 3] * fac);
+            w[e] = codes4<true>(acc[16 * c + 4 * e], acc[16 * c + 4 * e + 1], acc[16 * c + 4 * e + 2],
+                                acc[16 * c + 4 * e + 3], os, fac);
           code[c] = make_uint4(w[0], w[1], w[2], w[3]);
         }
         if (col0 + 64 > p.n && p.n % 16 != 0) {
@@ -1026,7 +1026,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float sc = fp8_scale(warp_max_nan(a)), fac = fp8_factor(sc);
           if (lane == 0) p.out_scales[row * p.ldos + f0 / kFp8Block] = sc;
           store_codes4(static_cast<uint8_t*>(p.out) + row * p.ldo + col, p.n - col,
-                       pack_e4m3x4(v.x * fac, v.y * fac, v.z * fac, v.w * fac));
+                       codes4<false>(v.x, v.y, v.z, v.w, sc, fac));
         } else {
           store4(static_cast<OutT*>(p.out) + row * p.ldo + col, left, v);
         }

@@ -193,37 +193,15 @@ __device__ __forceinline__ void put8(T* p, int left, const Eight& x) {
     }
   }
 }
-// The codes of eight values over their scale s, f = 1 / s: the product with f
-// corrected by its remainder (Markstein's step), so the code is that of the
-// rounded quotient and a tie between two codes stays one.  (With the product
-// alone, one code in 10^5 of 16-bit values is the other neighbour of a tie.)
-// Two at a time where registers allow (rows of f16, m = 16384, k = 768: 8.4 ->
-// 8.0 us; 7.7 without the correction); the norm, which is out of them, takes one
-// (bf16, m = 4095, k = 5000: 32.9 us, 33.7 by twos).
-template <bool TWO>
-__device__ __forceinline__ float2 quotients(float x, float y, float s, float f) {
-  float2 q;
-  if constexpr (TWO) {
-    asm("{\n\t.reg .b64 v, s, f, q, r;\n\t"
-        "mov.b64 v, {%2, %3};\n\tmov.b64 s, {%4, %4};\n\tmov.b64 f, {%5, %5};\n\t"
-        "mul.rn.f32x2 q, v, f;\n\tfma.rn.f32x2 r, q, s, v;\n\tfma.rn.f32x2 q, r, f, q;\n\t"
-        "mov.b64 {%0, %1}, q;\n\t}"
-        : "=f"(q.x), "=f"(q.y)
-        : "f"(x), "f"(y), "f"(-s), "f"(f));
-  } else {
-    q = make_float2(x * f, y * f);
-    q.x = __fmaf_rn(__fmaf_rn(-q.x, s, x), f, q.x);
-    q.y = __fmaf_rn(__fmaf_rn(-q.y, s, y), f, q.y);
-  }
-  return q;
-}
+// The codes of eight values over their scale s, f = 1 / s.  Two quotients at a
+// time where registers allow (rows of f16, m = 16384, k = 768: 8.4 -> 8.0 us; 7.7
+// with products by f alone); the norm, which is out of them, takes one (bf16, m =
+// 4095, k = 5000: 32.9 us, 33.7 by twos).
 template <bool VEC, bool APART, bool TWO>
 __device__ __forceinline__ void put_codes8(uint8_t* p, int left, const Eight& x, float s, float f) {
   constexpr int d = kSecond<APART>;
-  float2 q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = quotients<TWO>(x.v[2 * i], x.v[2 * i + 1], s, f);
-  const uint32_t a = pack_e4m3x4(q[0].x, q[0].y, q[1].x, q[1].y), b = pack_e4m3x4(q[2].x, q[2].y, q[3].x, q[3].y);
+  const uint32_t a = codes4<TWO>(x.v[0], x.v[1], x.v[2], x.v[3], s, f),
+                 b = codes4<TWO>(x.v[4], x.v[5], x.v[6], x.v[7], s, f);
   if (!APART && left >= 8) {
     *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
   } else if (!VEC) {
