@@ -71,8 +71,15 @@ int wc_fp8_gated_matmul(const void* d_a, int64_t lda, const float* d_sa, int64_t
 
 /* Waits for `stream` and reports what the products' kernels could not report
  * when they were enqueued: WC_E_TIMEOUT when an in-kernel wait ran out on the
- * current device since the last call (its results are then incomplete). */
+ * current device, on any of its streams, since the last call (the results of
+ * that product are then incomplete).  One call reports it, of whichever thread
+ * and stream: who runs products on several streams waits for all of them before
+ * any result is trusted.  No other call reports it. */
 int wc_fp8_sync(void* stream);
+
+/* Failure-detection self-test: enqueues a wait that nothing ends, as a product's
+ * would, and that gives up after limit_ns (1e6 .. 1e10); wc_fp8_sync reports it. */
+int wc_selftest_fp8_timeout(uint64_t limit_ns, void* stream);
 
 const char* wc_fp8_last_error(void);
 

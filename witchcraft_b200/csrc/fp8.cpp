@@ -238,7 +238,12 @@ extern "C" int wc_fp8_gated_matmul(const void* d_a, int64_t lda, const float* d_
 extern "C" int wc_fp8_sync(void* stream) {
   uint32_t s = 0;
   cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
-  if (e == cudaSuccess) e = fp8_gemm_take_status(&s);
+  if (e == cudaSuccess) e = fp8_gemm_take_status(&s, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return done(e, "synchronising");
   return s ? refuse(WC_E_TIMEOUT, "an in-kernel wait timed out") : WC_OK;
+}
+
+extern "C" int wc_selftest_fp8_timeout(uint64_t limit_ns, void* stream) {
+  if (limit_ns < 1000000ull || limit_ns > 10000000000ull) return refuse(WC_E_INVALID_ARG, "limit_ns must be 1e6 .. 1e10");
+  return done(fp8_gemm_timeout_selftest(limit_ns, static_cast<cudaStream_t>(stream)), "self-test launch");
 }

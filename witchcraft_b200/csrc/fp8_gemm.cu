@@ -1057,6 +1057,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 }  // namespace tile
 
+// ---------------------------------------------------------------- status
+
+__device__ uint32_t g_fp8_taken;  // what the last take_status_kernel found
+
+// Reads and clears in one step: a wait of another stream that runs out meanwhile
+// is either in what this one takes or left for the next.
+__global__ void take_status_kernel() { g_fp8_taken = atomicExch(&g_fp8_status, 0u); }
+
+// A wait that nothing ends, as a product's would run out.
+__global__ void timeout_selftest_kernel(uint64_t limit_ns) {
+  __shared__ uint64_t bar;
+  mbar_init(&bar, 1);
+  mbar_fence_init();
+  mbar_wait_limit(&bar, 0, &g_fp8_status, limit_ns);
+}
+
 // ---------------------------------------------------------------- host
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -1280,11 +1296,19 @@ cudaError_t fp8_gemm_launch(bool gated, int out_type, const Fp8GemmParams& p, in
   }
 }
 
-cudaError_t fp8_gemm_take_status(uint32_t* status) {
-  cudaError_t e = cudaMemcpyFromSymbol(status, g_fp8_status, sizeof(uint32_t));
-  if (e != cudaSuccess || *status == 0) return e;
-  const uint32_t zero = 0;
-  return cudaMemcpyToSymbol(g_fp8_status, &zero, sizeof(zero));
+cudaError_t fp8_gemm_take_status(uint32_t* status, cudaStream_t st) {
+  static std::mutex mu;  // one caller at a time has g_fp8_taken
+  std::lock_guard<std::mutex> lock(mu);
+  take_status_kernel<<<1, 1, 0, st>>>();
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(status, g_fp8_taken, sizeof(uint32_t), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  return e;
+}
+
+cudaError_t fp8_gemm_timeout_selftest(uint64_t limit_ns, cudaStream_t st) {
+  timeout_selftest_kernel<<<1, 1, 0, st>>>(limit_ns);
+  return cudaGetLastError();
 }
 
 }  // namespace wc

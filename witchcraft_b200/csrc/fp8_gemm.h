@@ -22,7 +22,11 @@ struct Fp8GemmParams {
 // out_type WC_T_E4M3 only with gated.
 cudaError_t fp8_gemm_launch(bool gated, int out_type, const Fp8GemmParams& p, int num_sms, cudaStream_t st);
 
-// The library's own status word on the current device, read and cleared.
-cudaError_t fp8_gemm_take_status(uint32_t* status);
+// The library's own status word on the current device, read and cleared in one
+// step on st; waits for it.
+cudaError_t fp8_gemm_take_status(uint32_t* status, cudaStream_t st);
+
+// Enqueues a wait that runs out after limit_ns and says so in that word.
+cudaError_t fp8_gemm_timeout_selftest(uint64_t limit_ns, cudaStream_t st);
 
 }  // namespace wc

@@ -95,7 +95,10 @@ def gated_matmul(a: torch.Tensor, a_scales: torch.Tensor, gate: torch.Tensor, ga
 
 def synchronize(device=None) -> None:
     """Waits for the current stream of `device`; raises if a product's
-    in-kernel wait ran out since the last call."""
+    in-kernel wait ran out on the device, on any stream, since the last call.
+
+    No other call reports that: call this before results are used, once every
+    stream with products has been waited for."""
     with torch.cuda.device(device):
         rc = lib().wc_fp8_sync(torch.cuda.current_stream().cuda_stream)
         if rc != 0:
