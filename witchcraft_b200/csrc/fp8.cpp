@@ -32,13 +32,13 @@ int type_size(int t) { return t == WC_T_F32 ? 4 : t == WC_T_E4M3 ? 1 : 2; }
 bool aligned(const void* p, int64_t ld, int bytes, int type) {  // rows start at multiples of `bytes`
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (ld * type_size(type)) % bytes == 0;
 }
-// rows of eight elements at a time: 16-byte accesses
 // Whether rows of n results can be written by TMA boxes, which end a row at a
 // multiple of 16 bytes: a row that ends between two would take the bytes behind
 // it along (zeros there).
 bool boxes(const void* p, int64_t ld, int64_t n, int type) {
   return aligned(p, ld, 16, type) && n * type_size(type) % 16 == 0;
 }
+// rows of eight elements at a time: 16-byte accesses
 bool vec8(const void* p, int64_t ld, int type) { return aligned(p, ld, 16, type) && ld % 8 == 0; }
 bool natural(const void* p, int type) { return reinterpret_cast<uintptr_t>(p) % type_size(type) == 0; }
 int64_t blocks(int64_t k) { return (k + 127) / 128; }

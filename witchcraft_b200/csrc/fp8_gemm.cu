@@ -54,7 +54,7 @@ constexpr int kThreads = 384;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kABytes = kRows * kFp8Block;
 
-__device__ uint32_t g_fp8_status;  // wait timeouts of launches without a status word of their own
+__device__ uint32_t g_fp8_status;  // wait timeouts
 
 // Instruction descriptor for kind::f8f6f4 with e4m3 A and B (format 0), f32
 // D, both K-major.
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* res_full = acc_empty + 2;    // [8][kBoxes] each epilogue warp's boxes of the residual
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + 8 * kBoxes);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  uint32_t* status = p.status ? p.status : &g_fp8_status;
+  uint32_t* status = &g_fp8_status;
   // a cluster is two neighbours of the grid; said with blockIdx, the compiler
   // knows that what follows from it is the same for the whole warp
   const int rank = blockIdx.x & 1;
@@ -892,7 +892,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* acc_empty = done + PL::kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + PL::kBufs);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  uint32_t* status = p.status ? p.status : &g_fp8_status;
+  uint32_t* status = &g_fp8_status;
 
   constexpr int kFeat = GATED ? BN / 2 : BN;
   const int kblocks = (p.k + kFp8Block - 1) / kFp8Block;
@@ -953,7 +953,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (q * 32 < rows) {
       const uint32_t tlane = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * (BN / 2);
       const int lrow = q * 32 + lane, row = m0 + lrow;
-      const int nb = f0 / kFp8Block + (GATED || BN == 128 ? 0 : h);  // block of weight rows
+      const int nb = f0 / kFp8Block;  // block of weight rows
       const int blocks = (kblocks - rank + split - 1) / split;  // at least one: split <= kblocks
       Scales sc = scales_at<GATED>(p, row, nb, rank);
       float acc[32 * kChunks];

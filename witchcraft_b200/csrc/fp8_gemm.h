@@ -16,13 +16,12 @@ struct Fp8GemmParams {
   int m, n, k;
   int act;                           // WC_ACT_*, gated only
   bool box_o, box_r;                 // rows of 16-byte blocks: whole ones of the output, aligned ones of the residual
-  uint32_t* status;                  // wait timeouts; null: the library's own word
 };
 
 // out_type WC_T_E4M3 only with gated.
 cudaError_t fp8_gemm_launch(bool gated, int out_type, const Fp8GemmParams& p, int num_sms, cudaStream_t st);
 
-// The library's own status word on the current device, read and cleared in one
+// The products' status word on the current device, read and cleared in one
 // step on st; waits for it.
 cudaError_t fp8_gemm_take_status(uint32_t* status, cudaStream_t st);
 
