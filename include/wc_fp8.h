@@ -81,6 +81,13 @@ int wc_fp8_sync(void* stream);
  * would, and that gives up after limit_ns (1e6 .. 1e10); wc_fp8_sync reports it. */
 int wc_selftest_fp8_timeout(uint64_t limit_ns, void* stream);
 
+/* Self-test of the choice between the products' kernels: how many CTAs share a
+ * tile (1, 2, 4 or 8: few rows), or 0 for tiles on pairs of SMs (many rows), in
+ * wc_fp8_matmul or wc_fp8_gated_matmul (gated) with these arguments.  residual:
+ * there is one; boxes: results and residual have rows of whole 16-byte blocks.
+ * Negative: a return code. */
+int wc_selftest_fp8_split(int gated, int64_t m, int64_t k, int64_t n, int out_type, int residual, int boxes);
+
 const char* wc_fp8_last_error(void);
 
 #ifdef __cplusplus

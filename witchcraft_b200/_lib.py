@@ -78,6 +78,7 @@ _SIGNATURES = {
                                     c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p,
                                     c_int, c_int64, c_void_p, c_int64, c_void_p]),
     "wc_fp8_sync": (c_int, [c_void_p]),
+    "wc_selftest_fp8_split": (c_int, [c_int, c_int64, c_int64, c_int64, c_int, c_int, c_int]),
     "wc_selftest_fp8_timeout": (c_int, [ctypes.c_uint64, c_void_p]),
     "wc_fp8_last_error": (ctypes.c_char_p, []),
 }

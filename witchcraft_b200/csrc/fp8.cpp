@@ -247,3 +247,18 @@ extern "C" int wc_selftest_fp8_timeout(uint64_t limit_ns, void* stream) {
   if (limit_ns < 1000000ull || limit_ns > 10000000000ull) return refuse(WC_E_INVALID_ARG, "limit_ns must be 1e6 .. 1e10");
   return done(fp8_gemm_timeout_selftest(limit_ns, static_cast<cudaStream_t>(stream)), "self-test launch");
 }
+
+extern "C" int wc_selftest_fp8_split(int gated, int64_t m, int64_t k, int64_t n, int out_type, int residual, int boxes) {
+  if (!sizes_ok(m, k, n) || m == 0) return refuse(WC_E_INVALID_ARG, "sizes out of range (m, k, n >= 1)");
+  if (!value_type(out_type) && !(gated && out_type == WC_T_E4M3)) return refuse(WC_E_INVALID_ARG, "unknown output type");
+  Fp8GemmParams p{};
+  p.m = static_cast<int>(m);
+  p.n = static_cast<int>(n);
+  p.k = static_cast<int>(k);
+  p.residual = residual && !gated ? &p : nullptr;  // only whether there is one counts
+  p.box_o = p.box_r = boxes != 0;
+  int sms = 0, split = 0;
+  if (const int rc = sm_count(&sms); rc != WC_OK) return rc;
+  const int rc = done(fp8_gemm_split(gated != 0, out_type, p, sms, &split), "choice of a kernel");
+  return rc != WC_OK ? rc : split;
+}

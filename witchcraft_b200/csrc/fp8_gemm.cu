@@ -1230,9 +1230,20 @@ struct Cost {  // us
   float tile, tile_rows, block, join, pair_start, pair_round, pair_block;
 };
 
+// Whether rows of results or of the residual start off the 16-byte boundary.
+template <typename OutT>
+bool off_boundary(const Fp8GemmParams& p) {
+  return sizeof(OutT) > 1 && !(p.box_o && (!p.residual || p.box_r));
+}
+
+// Columns of a single tile's weights: 128 features, of both in the gated product.
+template <bool GATED>
+constexpr int kTileBN = GATED ? 256 : 128;
+
+// CTAs that share a single tile's K, or 0 for pairs of SMs.
 template <bool GATED, typename OutT>
-cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
-  constexpr int BN = GATED ? 256 : 128;
+cudaError_t choose(const Fp8GemmParams& p, int num_sms, int* chosen) {
+  constexpr int BN = kTileBN<GATED>;
   constexpr int kFeat = 128;  // output columns of a single tile
   const int64_t kblocks = (static_cast<int64_t>(p.k) + kFp8Block - 1) / kFp8Block;
   const int64_t tiles = static_cast<int64_t>((p.m + kRows - 1) / kRows) * ((p.n + kFeat - 1) / kFeat);
@@ -1249,7 +1260,7 @@ cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
   const float rows = static_cast<float>(std::min<int64_t>(p.m, kRows)) / kRows;
   constexpr int kPairFeat = GATED ? 128 : 256;
   const int64_t pairs = static_cast<int64_t>((p.m + 2 * kRows - 1) / (2 * kRows)) * ((p.n + kPairFeat - 1) / kPairFeat);
-  const bool off = sizeof(OutT) > 1 && !(p.box_o && (!p.residual || p.box_r));
+  const bool off = off_boundary<OutT>(p);
   const float pair_off = !off ? 0.0f : (p.residual ? 3.2f : 1.3f) * (sizeof(OutT) == 4 ? 1.6f : 1.0f);
   const float tile_res = !p.residual ? 0.0f : rows * (off ? 3.0f : 1.2f) * (sizeof(OutT) == 4 ? 2.0f : 1.0f);
   float best = c.pair_start + static_cast<float>((pairs + clusters_of(num_sms) - 1) / clusters_of(num_sms)) *
@@ -1268,9 +1279,18 @@ cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
       split = s;
     }
   }
+  *chosen = split;
+  return cudaSuccess;
+}
+
+template <bool GATED, typename OutT>
+cudaError_t launch(const Fp8GemmParams& p, int num_sms, cudaStream_t st) {
+  constexpr int BN = kTileBN<GATED>;
+  int split = 0;
+  if (cudaError_t e = choose<GATED, OutT>(p, num_sms, &split); e != cudaSuccess) return e;
   if (split == 0) {
     if constexpr (sizeof(OutT) > 1)
-      if (off) return launch_pair<GATED, OutT, false>(p, num_sms, st);
+      if (off_boundary<OutT>(p)) return launch_pair<GATED, OutT, false>(p, num_sms, st);
     return launch_pair<GATED, OutT, true>(p, num_sms, st);
   }
   return p.m <= 32 ? launch_tile<GATED, OutT, BN, 32>(p, split, st) : launch_tile<GATED, OutT, BN, kRows>(p, split, st);
@@ -1292,6 +1312,24 @@ cudaError_t fp8_gemm_launch(bool gated, int out_type, const Fp8GemmParams& p, in
     case WC_T_F32: return launch<false, float>(p, num_sms, st);
     case WC_T_F16: return launch<false, __half>(p, num_sms, st);
     case WC_T_BF16: return launch<false, __nv_bfloat16>(p, num_sms, st);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t fp8_gemm_split(bool gated, int out_type, const Fp8GemmParams& p, int num_sms, int* split) {
+  if (gated) {
+    switch (out_type) {
+      case WC_T_F32: return choose<true, float>(p, num_sms, split);
+      case WC_T_F16: return choose<true, __half>(p, num_sms, split);
+      case WC_T_BF16: return choose<true, __nv_bfloat16>(p, num_sms, split);
+      case WC_T_E4M3: return choose<true, uint8_t>(p, num_sms, split);
+      default: return cudaErrorInvalidValue;
+    }
+  }
+  switch (out_type) {
+    case WC_T_F32: return choose<false, float>(p, num_sms, split);
+    case WC_T_F16: return choose<false, __half>(p, num_sms, split);
+    case WC_T_BF16: return choose<false, __nv_bfloat16>(p, num_sms, split);
     default: return cudaErrorInvalidValue;
   }
 }

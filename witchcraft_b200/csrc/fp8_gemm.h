@@ -21,6 +21,9 @@ struct Fp8GemmParams {
 // out_type WC_T_E4M3 only with gated.
 cudaError_t fp8_gemm_launch(bool gated, int out_type, const Fp8GemmParams& p, int num_sms, cudaStream_t st);
 
+// Which kernel fp8_gemm_launch takes: CTAs that share a tile, 0 for pairs of SMs.
+cudaError_t fp8_gemm_split(bool gated, int out_type, const Fp8GemmParams& p, int num_sms, int* split);
+
 // The products' status word on the current device, read and cleared in one
 // step on st; waits for it.
 cudaError_t fp8_gemm_take_status(uint32_t* status, cudaStream_t st);
