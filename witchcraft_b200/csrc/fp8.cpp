@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "../../include/wc_fp8.h"
 #include "../../include/wc_t5cuda.h"
 #include "fp8_gemm.h"
@@ -63,7 +65,7 @@ const char* check_values(const void* p, int type, int64_t ld, int64_t k) {
 }
 
 int sm_count(int* n) {
-  static int counts[64] = {};
+  static std::atomic<int> counts[64] = {};  // calls come from any thread
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return done(e, "device");

@@ -43,6 +43,7 @@
 #include "fp8_span.h"
 
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 
 namespace wc {
@@ -1126,7 +1127,7 @@ bool values_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int
 // Largest dynamic shared memory, once per device and kernel.
 template <auto KERNEL>
 cudaError_t allow_smem(int bytes) {
-  static bool set[64] = {};
+  static std::atomic<bool> set[64] = {};  // calls come from any thread
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -1204,10 +1205,11 @@ cudaError_t launch_tile(const Fp8GemmParams& p, int split, cudaStream_t st) {
 // cluster stays inside a group of SMs, so large ones leave some of them idle.
 template <auto KERNEL>
 int resident_ctas(int split, int smem, int num_sms) {
-  static int counts[64][4] = {};
+  static std::atomic<int> counts[64][4] = {};  // calls come from any thread
   int dev = 0;
   if (split == 1 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return num_sms;
-  int& n = counts[dev][split == 2 ? 1 : split == 4 ? 2 : 3];
+  std::atomic<int>& count = counts[dev][split == 2 ? 1 : split == 4 ? 2 : 3];
+  int n = count.load();
   if (n == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(num_sms / split * split));
@@ -1222,6 +1224,7 @@ int resident_ctas(int split, int smem, int num_sms) {
       clusters = num_sms / split;
     }
     n = std::max(split, clusters * split);
+    count.store(n);
   }
   return n;
 }
