@@ -8,8 +8,8 @@
  * A value is code * scale.  Rows (activations) have one scale per row and
  * 128 columns: scales [rows][ceil(k / 128)]; weights one per 128 x 128
  * block: scales [ceil(n / 128)][ceil(k / 128)].  The scale of a block is
- * max(max|x| / 448, 2^-126), its codes x / scale rounded to the nearest e4m3
- * value (ties to even) and saturated.  A block that holds a NaN or an
+ * max(max|x| / 448, 2^-126), its codes x / scale (the rounded f32 quotient)
+ * rounded to the nearest e4m3 value (ties to even) and saturated.  A block that holds a NaN or an
  * infinity gets a NaN or infinite scale and stands for NaN throughout.
  *
  * Codes start at 16-byte boundaries and so do their rows (the leading

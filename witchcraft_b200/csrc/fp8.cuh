@@ -13,8 +13,8 @@ constexpr int kFp8Block = 128;      // columns (and weight rows) that share a sc
 constexpr float kE4M3Max = 448.0f;  // largest finite e4m3 value
 
 // The scale of a block whose largest magnitude is amax (NaN stays NaN): the
-// product with 1 / 448 corrected by its remainder, the rounded quotient but
-// for rare last bits.  The floor keeps the reciprocal finite; a block of zeros
+// product with 1 / 448 corrected by its remainder, which is the rounded quotient
+// for every fraction of amax.  The floor keeps the reciprocal finite; a block of zeros
 // gets codes of zero.
 __device__ __forceinline__ float fp8_scale(float amax) {
   constexpr float c = 1.0f / kE4M3Max;

@@ -24,11 +24,12 @@
 // What bounds them (device time, inputs from DRAM).  Many rows: the epilogue
 // warps, which both add up the partials and finish the tile before.  8192 x 4096
 // x 8192, f16: 240 to 270 us, 2.0 to 2.3 PFLOP/s as the clock under power
-// allows; 2048 x 4096 x 4096: 33.2 us, 28.3 if the tensor core could sum all of
-// K (no scales).  Gated 16384 x 768 x 2048 to 8-bit rows: 65 to 75 us, where the
+// allows; 2048 x 4096 x 4096: 33.5 us, 28.3 if the tensor core could sum all of
+// K (no scales).  Gated 16384 x 768 x 2048 to 8-bit rows: 68 to 76 us, where the
 // tensor pipe works 35 % and the schedulers issue 57 % of the time.  Few rows:
 // latency (32 x 768 x 2304: 4.2 us, of which 1 is a launch that does nothing much), and
-// for one row of 4096 x 12288 the weights, 12.9 us or 3.9 TB/s.
+// for one row of 4096 x 12288 the 96 CTAs (of 148 SMs) that its tiles make,
+// 12.9 us or 3.9 TB/s of weights.
 //
 // Warps of both (384 threads):
 //   0      TMA producer, 128-byte swizzle, ring of operand stages
@@ -1257,7 +1258,7 @@ cudaError_t choose(const Fp8GemmParams& p, int num_sms, int* chosen) {
   // A pair's round is cheaper per element but starts slower, and rows off the
   // 16-byte boundary cost it more than the single tile, whose CTAs also share the
   // residual's rows.  Measured with 768 <= k <=
-  // 8192, 1 <= m <= 4096; at m = 128, k = 768, n = 2304: 6.1 / 6.8 / 5.6 / 6.5 us
+  // 8192 and 1 <= m <= 4096, extrapolated elsewhere; at m = 128, k = 768, n = 2304: 6.1 / 6.8 / 5.6 / 6.5 us
   // with 1, 2, 4, 8 CTAs a tile and 6.8 on pairs.
   const Cost c = GATED ? Cost{2.8f, 4.2f, 0.46f, 0.6f, 2.8f, 1.8f, 0.45f} : Cost{2.05f, 1.95f, 0.32f, 0.65f, 4.0f, 1.0f, 0.42f};
   const float rows = static_cast<float>(std::min<int64_t>(p.m, kRows)) / kRows;

@@ -103,8 +103,9 @@ __device__ __forceinline__ uint2 four_16bit(const uint16_t* e, int left) {
   return make_uint2((left > 0 ? e[0] : 0u) | (left > 1 ? e[1] : 0u) << 16, left > 2 ? e[2] : 0u);
 }
 // The lane's runs at p, `left` columns of the row being left from there on;
-// zeros past it.  Each is read once: marked to be evicted first (norm m = 16384,
-// k = 768: 30.2 -> 28.8 us).
+// zeros past it.  Rows are read once and marked to be evicted first (norm m =
+// 16384, k = 768: 30.2 -> 28.8 us); the norm weights, which every row reads, and
+// the first pass over rows wider than a CTA's registers go the same way.
 template <bool VEC, bool APART, typename T>
 __device__ __forceinline__ Raw8<T> get8(const T* p, int left) {
   constexpr int d = kSecond<APART>;
@@ -250,9 +251,10 @@ __global__ void __launch_bounds__(32 * kWarps) fp8_rows_kernel(const __grid_cons
 
 // One row by WPR warps, its kHeld units per warp in registers between the sum
 // of squares and the scaling (rows up to WPR * kHeld * 256 columns).  Five CTAs
-// an SM at 48 registers (norm m = 16384, k = 768: 27.1 us with four, 26.2 with
-// five, 34.3 with six, which spill): the loads of one row overlap the
-// arithmetic of the others.
+// an SM at 48 registers (norm m = 16384, k = 768 with an f16 residual: 27.1 us
+// with four, 26.2 with five, 34.3 with six, which spill): the loads of one row
+// overlap the arithmetic of the others.  With f32 rows and an f32 residual five
+// spill too, 32 to 64 bytes a thread (33.4 us, 4.9 TB/s).
 template <typename TX, typename TD, bool DELTA, bool VEC, int WPR>
 __global__ void __launch_bounds__(32 * kWarps, 5) fp8_rmsnorm_kernel(const __grid_constant__ Fp8RowsParams p) {
   __shared__ float part[kWarps];
